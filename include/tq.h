@@ -31,7 +31,7 @@ extern "C" {
 #define TQ_ERR_ALIGN (-3)       /* pointer not aligned as the entry point requires */
 #define TQ_ERR_HIP (-4)         /* HIP runtime error (no device, launch failure)   */
 
-enum { TQ_F16 = 0, TQ_F32 = 1, TQ_F64 = 2 };
+enum { TQ_F16 = 0, TQ_F32 = 1, TQ_F64 = 2, TQ_BF16 = 3 }; /* TQ_BF16: where an entry point says so */
 enum { TQ_ROT_DENSE = 0, TQ_ROT_WHT = 1 };
 enum { TQ_KIND_K = 0, TQ_KIND_V = 1 };
 enum { TQ_DOMAIN_ROTATED = 0, TQ_DOMAIN_ORIGINAL = 1 };
@@ -416,6 +416,31 @@ int tq_decode_attention_static(const tq_handle *hk, const tq_handle *hv, const t
 int tq_score_tile(const tq_handle *h, const void *q, int q_dtype, int64_t nq, const void *packed,
                   const uint8_t *sign_bits, const void *rnorms_f16, int64_t nk, void *logits, int out_dtype,
                   void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- rotary positions ---------------------------------------------------------- */
+
+/* Queries and keys turned to their positions: of every head's first rotary_dim values, pair i (values i and i + rotary_dim / 2,
+ * or 2 i and 2 i + 1 with `interleaved`) becomes
+ *     (u cos a - w sin a, w cos a + u sin a) * magnitude,   a = 2 pi turns[i] * position,
+ * and the others are taken over.  `inverse` turns by -a, which is also the gradient of the call without it.  No counterpart in
+ * the reference, whose keys arrive rotated; this comes before tq_append_paged and tq_paged_attention. */
+typedef struct tq_rotary_params {
+    int64_t tokens;
+    int32_t n_q_heads, n_k_heads;       /* 0 heads: that tensor is left out and its pointers may be NULL          */
+    int32_t head_dim;                   /* 1 .. 65536                                                              */
+    int32_t rotary_dim;                 /* even, 2 .. head_dim, at most 1024                                       */
+    int32_t interleaved, inverse;
+    int32_t dtype;                      /* TQ_F16 | TQ_F32 | TQ_BF16 of q and k and of what is written             */
+    int32_t positions_64;               /* positions are int64 (else int32); any value                             */
+    float magnitude;
+    int64_t q_token, q_head, k_token, k_head;                 /* strides in values; those of a head's values are 1  */
+    int64_t q_out_token, q_out_head, k_out_token, k_out_head;
+} tq_rotary_params;
+/* q, k: [tokens, heads, head_dim] by their strides; turns: [rotary_dim / 2] float64 in device memory, turns of a pair per position
+ * (angles are reduced in 64 bits: a position of 2^31 is as exact as 1).  q_out may be q, and k_out k, with the same
+ * strides; otherwise what is written must not overlap what is read.  Pointers need the alignment of their type. */
+int tq_rotary(const tq_rotary_params *p, const void *q, void *q_out, const void *k, void *k_out, const void *positions,
+              const double *turns, void *stream);
 
 /* Large host arrays by several of the caller's threads.  A board and a job lie in the caller's memory, zeroed but for the job's
  * first six fields (up to `slots`).

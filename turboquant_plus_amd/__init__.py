@@ -11,6 +11,7 @@ from .turboquant import TurboQuant, TurboQuantMSE, CompressedVector
 from .kv_cache import KVCacheCompressor, CompressedKVCache
 from .outlier import OutlierTurboQuant, OutlierCompressedVector
 from .policy import LayerFormat, LayerKV, layer_formats, effective_bits
+from .rotary import Rotary, RotaryScaling, rotary_frequencies
 from .turbo import (TurboCodec, DecodeAttention, q8_0_store, q8_0_unpack, q8_0_append, packed_bytes, PRODUCTION_CENTROIDS,
                     sparse_bias_from_dense, rows_of_256)
 
@@ -18,4 +19,4 @@ __all__ = ["PolarQuant", "QJL", "TurboQuant", "TurboQuantMSE", "CompressedVector
            "OutlierTurboQuant", "OutlierCompressedVector",
            "CompressedKVCache", "TurboCodec", "DecodeAttention", "q8_0_store", "q8_0_unpack", "q8_0_append", "packed_bytes",
            "PRODUCTION_CENTROIDS", "sparse_bias_from_dense", "rows_of_256", "LayerFormat", "LayerKV", "layer_formats",
-           "effective_bits"]
+           "effective_bits", "Rotary", "RotaryScaling", "rotary_frequencies"]

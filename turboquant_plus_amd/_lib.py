@@ -19,7 +19,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # `make KNOCKOUT=.. OUT=..` produces); unset, the product library next to this file is loaded.
 LIB_PATH = os.environ.get("TQ_HIP_LIBRARY") or os.path.join(_HERE, "libtq_hip.so")
 
-TQ_F16, TQ_F32, TQ_F64 = 0, 1, 2
+TQ_F16, TQ_F32, TQ_F64, TQ_BF16 = 0, 1, 2, 3
 ROT_DENSE, ROT_WHT = 0, 1
 KIND_K, KIND_V = 0, 1
 DOMAIN_ROTATED, DOMAIN_ORIGINAL = 0, 1
@@ -45,6 +45,14 @@ class TQAttnParams(C.Structure):
 class TQAttnPlan(C.Structure):
     _fields_ = [("passes", C.c_int32), ("heads_per_pass", C.c_int32), ("wavefronts", C.c_int32), ("partials", C.c_int32),
                 ("groups_per_workgroup", C.c_int32), ("lane_tables", C.c_int32), ("workgroups", C.c_int64)]
+
+
+class TQRotaryParams(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("n_q_heads", C.c_int32), ("n_k_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("inverse", C.c_int32), ("dtype", C.c_int32),
+                ("positions_64", C.c_int32), ("magnitude", C.c_float), ("q_token", C.c_int64), ("q_head", C.c_int64),
+                ("k_token", C.c_int64), ("k_head", C.c_int64), ("q_out_token", C.c_int64), ("q_out_head", C.c_int64),
+                ("k_out_token", C.c_int64), ("k_out_head", C.c_int64)]
 
 
 HOST_SLOTS = 8
@@ -117,6 +125,7 @@ PROTOTYPES = {
     "tq_decode_attention_plan": (_I, [C.POINTER(TQAttnParams), _I, _I, _I, _I, _L, C.POINTER(TQAttnPlan)]),
     "tq_decode_attention": (_I, [_P, _P, C.POINTER(TQAttnParams), _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
     "tq_decode_attention_static": (_I, [_P, _P, C.POINTER(TQAttnParams), _P, _I, _P, _P, _P, _P, _P, _P]),
+    "tq_rotary": (_I, [C.POINTER(TQRotaryParams), _P, _P, _P, _P, _P, _P, _P]),
     "tq_host_serve": (None, [C.POINTER(TQHostBoard)]),
     "tq_host_open": (_I, [C.POINTER(TQHostBoard), _I]),
     "tq_host_close": (None, [C.POINTER(TQHostBoard), _I]),

@@ -8,7 +8,7 @@
 #include <limits>
 #include <vector>
 
-#include "tq_internal.h"
+#include "tq_check.h"
 
 namespace {
 
@@ -58,10 +58,6 @@ template <typename T> int upload(T **dst, const std::vector<T> &src) {
     }
     return TQ_OK;
 }
-
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-bool fast_ok(const tq_handle *h) { return h->d == 128 && h->rotation == TQ_ROT_WHT && h->s1_32; }
 
 }  // namespace
 
@@ -418,14 +414,6 @@ void tq_destroy(tq_handle *h) {
     delete h;
 }
 
-#define REQUIRE(cond, code, ...)      \
-    do {                              \
-        if (!(cond)) {                \
-            tq_set_error(__VA_ARGS__); \
-            return code;              \
-        }                             \
-    } while (0)
-
 int tq_fwht(const void *x, void *y, int64_t n, int32_t len, int in_dtype, int out_dtype, void *stream) {
     REQUIRE(n >= 0 && (n == 0 || (x && y)), TQ_ERR_ARG, "tq_fwht: bad argument");
     REQUIRE(len >= 1 && (len & (len - 1)) == 0, TQ_ERR_ARG, "Input length must be a positive power of 2, got %d", len);
@@ -520,14 +508,6 @@ int64_t tq_packed_bytes(int32_t bits, int64_t n_seqs, int64_t tokens) {
 int64_t tq_q8_0_bytes(int64_t n_seqs, int64_t tokens) {
     if (n_seqs < 0 || tokens < 0) return -1;
     return n_seqs * ((tokens + TQ_ROWS_PER_BLOCK - 1) / TQ_ROWS_PER_BLOCK) * (int64_t)(TQ_ROWS_PER_BLOCK * 136);
-}
-
-static int check_fast(const tq_handle *h, const char *who) {
-    REQUIRE(h, TQ_ERR_ARG, "%s: null handle", who);
-    REQUIRE(fast_ok(h), TQ_ERR_UNSUPPORTED, "%s: needs d == 128 and WHT rotation (handle has d=%d, rotation=%d)", who,
-            h->d, h->rotation);
-    REQUIRE(h->bits >= 2 && h->bits <= 4, TQ_ERR_UNSUPPORTED, "%s: bits must be 2, 3 or 4 (got %d)", who, h->bits);
-    return TQ_OK;
 }
 
 int tq_store(const tq_handle *h, const void *x, int64_t n_seqs, int64_t tokens, int in_dtype, int kind, void *packed,
