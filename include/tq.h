@@ -442,6 +442,66 @@ typedef struct tq_rotary_params {
 int tq_rotary(const tq_rotary_params *p, const void *q, void *q_out, const void *k, void *k_out, const void *positions,
               const double *turns, void *stream);
 
+/* ---- caches in pages ------------------------------------------------------------ */
+
+/* A page is a 128-token block of every KV head of a layer: a pool holds [n_pages, n_kv_heads, bytes of a block] (tq_packed_bytes(bits, 1,
+ * 128) or tq_q8_0_bytes(1, 128)), K and V in pools of their own under the same page numbers.  Position p of sequence b lies in page
+ * block_table[b * table_stride + p / 128], row p % 128.  Rows of new tokens are token-major, [rows, heads, 128], sequence after
+ * sequence: b's are cu_new[b] .. cu_new[b + 1] - 1 (cu_new NULL: one row each).  All tables are device memory, read when a
+ * launch runs, so one captured launch serves steps whose tables and lengths change.
+ * What they hold is checked there: a sequence whose rows lie outside 0 .. rows has none, and the pages of an entry outside
+ * 0 .. n_pages - 1 are neither read nor written.  No counterpart in the reference, whose cache is rebuilt whole
+ * (kv_cache.py:41-66). */
+typedef struct tq_pages {
+    int32_t batch, n_kv_heads;
+    int32_t n_pages;
+    int32_t max_blocks;         /* entries of a row of block_table, at most 2^24 - 1  */
+    int64_t table_stride;       /* from one sequence's row to the next                 */
+    const int32_t *block_table; /* [batch, max_blocks]                                 */
+    const int32_t *cu_new;      /* [batch + 1], not descending; or NULL                */
+    const int32_t *lens;        /* [batch]: tq_append_paged, tq_load_paged: position of the first row;   */
+                                /* tq_paged_attention: tokens that the cache holds, the new ones among them */
+} tq_pages;
+
+/* The rows k, v [rows, n_kv_heads, 128] (strides in values; a head's values are next to each other) quantised into their
+ * sequences' pages from position lens[b] on: in one launch, with the bytes that tq_append_layer writes.  hk / hv NULL: q8_0-style rows.
+ * As there, tokens before lens[b] stay and what follows the last new token in its block becomes the code of 0.0 with norm 0.
+ * in_dtype TQ_F16, TQ_BF16 or TQ_F32; codebooks must be symmetric (TQ_ERR_UNSUPPORTED).  Rows, strides and pages of turbo formats are
+ * 16-byte aligned.  A page that is written must belong to one sequence.  A sequence that starts below 0 or ends beyond max_blocks * 128
+ * writes nothing, nor does a block whose entry is no page; with overrun_dev (as in tq_append_kv_at) TQ_OVERRUN_NEGATIVE,
+ * TQ_OVERRUN_NO_ROOM or TQ_OVERRUN_NO_PAGE is set there. */
+#define TQ_OVERRUN_NO_PAGE 4u  /* an entry of block_table outside 0 .. n_pages - 1, or cu_new outside 0 .. rows */
+int tq_append_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *pages, const void *k, const void *v, int64_t rows,
+                    int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, int in_dtype, void *k_pages, void *v_pages,
+                    uint32_t *overrun_dev, void *stream);
+
+/* The inverse of tq_append_paged: positions lens[b] .. of every sequence back as fp16 values in the original domain, out_k and out_v
+ * [rows, n_kv_heads, 128], 16-byte aligned.  Rows behind the last sequence and rows without a page are left as they were. */
+int tq_load_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *pages, const void *k_pages, const void *v_pages, int64_t rows,
+                  void *out_k, void *out_v, void *stream);
+
+/* Attention of new tokens over a paged cache: for row t of the n of sequence b, which holds c = lens[b] tokens,
+ *     out = softmax(scale q K^T) V  over the positions before c - n + t + 1 (causal) or before c;
+ * a row that sees nothing is 0.  One row (a decode step), a few (drafted tokens), chunks and whole prompts; queries over another
+ * sequence's states with causal = 0. */
+typedef struct tq_paged_attn_params {
+    tq_pages pages;
+    int32_t n_q_heads;          /* a multiple of n_kv_heads; query head h reads KV head h / (n_q_heads / n_kv_heads) */
+    int32_t causal;
+    float scale;                /* positive                                                       */
+    int32_t dtype;              /* TQ_F16 | TQ_BF16 of q and out                                   */
+    int64_t rows;               /* of q and out, at least cu_new[batch]                            */
+    int64_t q_token, q_head;    /* strides of q in values, multiples of 8; out is [rows, n_q_heads, 128] */
+    int32_t max_context;        /* no sequence holds more (what lies behind is not seen); 0: max_blocks * 128        */
+    int32_t max_new;            /* no sequence has more rows (further ones are left as they were); 0: rows.  Both    */
+                                /* size the launch                                                                  */
+} tq_paged_attn_params;
+/* Bytes of workspace for these parameters (16-byte aligned; it may hold anything; calls that share one must not overlap in time). */
+int64_t tq_paged_attn_workspace_bytes(const tq_paged_attn_params *p);
+/* q, out and pages 16-byte aligned; hk / hv NULL: q8_0-style rows on that side.  Rows behind the last sequence are left as they were. */
+int tq_paged_attention(const tq_handle *hk, const tq_handle *hv, const tq_paged_attn_params *p, const void *q, const void *k_pages,
+                       const void *v_pages, void *out, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Large host arrays by several of the caller's threads.  A board and a job lie in the caller's memory, zeroed but for the job's
  * first six fields (up to `slots`).
  * Threads in tq_host_serve work on the jobs of a board and sleep between them; they return some milliseconds after its last user has

@@ -10,6 +10,7 @@ from .qjl import QJL
 from .turboquant import TurboQuant, TurboQuantMSE, CompressedVector
 from .kv_cache import KVCacheCompressor, CompressedKVCache
 from .outlier import OutlierTurboQuant, OutlierCompressedVector
+from .paged import PagedAttention, append_paged, load_paged, new_pages, page_bytes
 from .policy import LayerFormat, LayerKV, layer_formats, effective_bits
 from .rotary import Rotary, RotaryScaling, rotary_frequencies
 from .turbo import (TurboCodec, DecodeAttention, q8_0_store, q8_0_unpack, q8_0_append, packed_bytes, PRODUCTION_CENTROIDS,
@@ -19,4 +20,5 @@ __all__ = ["PolarQuant", "QJL", "TurboQuant", "TurboQuantMSE", "CompressedVector
            "OutlierTurboQuant", "OutlierCompressedVector",
            "CompressedKVCache", "TurboCodec", "DecodeAttention", "q8_0_store", "q8_0_unpack", "q8_0_append", "packed_bytes",
            "PRODUCTION_CENTROIDS", "sparse_bias_from_dense", "rows_of_256", "LayerFormat", "LayerKV", "layer_formats",
-           "effective_bits", "Rotary", "RotaryScaling", "rotary_frequencies"]
+           "effective_bits", "Rotary", "RotaryScaling", "rotary_frequencies", "PagedAttention", "append_paged",
+           "load_paged", "new_pages", "page_bytes"]

@@ -55,6 +55,16 @@ class TQRotaryParams(C.Structure):
                 ("k_out_token", C.c_int64), ("k_out_head", C.c_int64)]
 
 
+class TQPages(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("n_kv_heads", C.c_int32), ("n_pages", C.c_int32), ("max_blocks", C.c_int32),
+                ("table_stride", C.c_int64), ("block_table", C.c_void_p), ("cu_new", C.c_void_p), ("lens", C.c_void_p)]
+
+
+class TQPagedAttnParams(C.Structure):
+    _fields_ = [("pages", TQPages), ("n_q_heads", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float), ("dtype", C.c_int32),
+                ("rows", C.c_int64), ("q_token", C.c_int64), ("q_head", C.c_int64), ("max_context", C.c_int32), ("max_new", C.c_int32)]
+
+
 HOST_SLOTS = 8
 HOST_FETCH, HOST_WIDEN, HOST_UPLOAD, HOST_NARROW = 0, 1, 2, 3
 
@@ -126,6 +136,10 @@ PROTOTYPES = {
     "tq_decode_attention": (_I, [_P, _P, C.POINTER(TQAttnParams), _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
     "tq_decode_attention_static": (_I, [_P, _P, C.POINTER(TQAttnParams), _P, _I, _P, _P, _P, _P, _P, _P]),
     "tq_rotary": (_I, [C.POINTER(TQRotaryParams), _P, _P, _P, _P, _P, _P, _P]),
+    "tq_append_paged": (_I, [_P, _P, C.POINTER(TQPages), _P, _P, _L, _L, _L, _L, _L, _I, _P, _P, _P, _P]),
+    "tq_load_paged": (_I, [_P, _P, C.POINTER(TQPages), _P, _P, _L, _P, _P, _P]),
+    "tq_paged_attn_workspace_bytes": (_L, [C.POINTER(TQPagedAttnParams)]),
+    "tq_paged_attention": (_I, [_P, _P, C.POINTER(TQPagedAttnParams), _P, _P, _P, _P, _P, _L, _P]),
     "tq_host_serve": (None, [C.POINTER(TQHostBoard)]),
     "tq_host_open": (_I, [C.POINTER(TQHostBoard), _I]),
     "tq_host_close": (None, [C.POINTER(TQHostBoard), _I]),

@@ -1,0 +1,220 @@
+// Caches in pages: the C entry points, how an attention launch is laid out, and the join of its splits.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "tq_check.h"
+#include "tq_paged_attn.h"
+
+int tqk_paged_attn_k2(const tqpaged::PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s);
+int tqk_paged_attn_k3(const tqpaged::PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s);
+int tqk_paged_attn_k4(const tqpaged::PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s);
+int tqk_paged_attn_k8(const tqpaged::PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s);
+
+namespace {
+
+using namespace tqpaged;
+
+constexpr int MERGE_THREADS = 256;
+
+// The splits' partial results of a row -> its output: a wavefront per row and query head, two dims per lane.
+__global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedAttnArgs a) {
+    const int lane = threadIdx.x & 63, heads = a.r.p.n_kv_heads * a.group;
+    const int64_t at = (int64_t)blockIdx.x * (MERGE_THREADS / 64) + (threadIdx.x >> 6);
+    const int64_t row = at / heads;
+    const int head = (int)(at - row * heads);
+    if (row >= a.r.rows) return;
+    int b, nth;
+    if (!paged_item(a.r, (int)row, [&](int s) { return paged_seq(a.r, s).n; }, b, nth)) return;
+    const PagedSeq seq = paged_seq(a.r, b);
+    const PagedSpan span = paged_span(a, seq);
+    if (span.splits <= 1 || nth >= a.max_new) return;
+    const int64_t place = ((seq.row0 + nth) * heads + head) * a.n_splits;
+    float top = -INFINITY;
+    for (int s = lane; s < span.splits; s += 64) top = fmaxf(top, a.part_ml[2 * (place + s)]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float off = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < span.splits; ++s) {
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (place + s));
+        const float2 v = *reinterpret_cast<const float2 *>(a.part_o + (place + s) * 128 + 2 * lane);
+        const float f = __builtin_amdgcn_exp2f(ml.x - off);
+        l = fmaf(ml.y, f, l);
+        o0 = fmaf(v.x, f, o0);
+        o1 = fmaf(v.y, f, o1);
+    }
+    float inv = l > 0.0f ? a.v_unscale / l : l == 0.0f ? 0.0f : l;
+    if (a.vs1) {
+        const float2 s1 = *reinterpret_cast<const float2 *>(a.vs1 + 2 * lane), s2 = *reinterpret_cast<const float2 *>(a.vs2 + 2 * lane);
+        o0 *= s2.x;
+        o1 *= s2.y;
+        wht128_wave(o0, o1, lane);
+        o0 *= s1.x;
+        o1 *= s1.y;
+        inv *= RSQRT128;
+    }
+    o0 *= inv;
+    o1 *= inv;
+    const uint32_t lo = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o0) : __builtin_bit_cast(uint16_t, (_Float16)o0);
+    const uint32_t hi = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o1) : __builtin_bit_cast(uint16_t, (_Float16)o1);
+    reinterpret_cast<uint32_t *>(a.out)[((seq.row0 + nth) * heads + head) * 64 + lane] = lo | (hi << 16);
+}
+
+struct Plan {
+    int rb, kw, n_splits, split_tiles, max_context, max_new;
+    int64_t items;   // row blocks of all sequences, an upper bound
+    unsigned grid;
+};
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool make_plan(const tq_paged_attn_params *p, Plan &pl) {
+    const int64_t group = p->n_q_heads / p->pages.n_kv_heads, rows = p->rows;
+    const int64_t max_new = p->pages.cu_new ? (p->max_new > 0 ? std::min<int64_t>(p->max_new, rows) : rows) : 1;
+    pl.max_new = (int)max_new;
+    const int64_t most = max_new * group;
+    pl.rb = most <= 16 ? 1 : most <= 32 ? 2 : 4;
+    const int64_t tile = 16 * pl.rb;
+    const int w = paged_waves(pl.rb);
+    pl.items = std::min(p->pages.batch * ceil_div(most, tile), rows * group / tile + p->pages.batch);
+    const int64_t room = (int64_t)p->pages.max_blocks * TQ_ROWS_PER_BLOCK;
+    pl.max_context = (int)(p->max_context > 0 ? std::min<int64_t>(p->max_context, room) : room);
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(pl.max_context, 64));
+    // wavefronts that fill the chip: two per SIMD, four where a wavefront has one block of rows
+    const int64_t want = pl.rb == 1 ? 4096 : 2048, blocks = pl.items * p->pages.n_kv_heads;
+    pl.kw = 1;
+    while (pl.kw < w && blocks * pl.kw < want && tiles >= 2 * pl.kw) pl.kw *= 2;
+    int64_t splits = std::max<int64_t>(1, std::min(ceil_div(want, blocks * pl.kw), tiles / (2 * pl.kw)));
+    pl.split_tiles = (int)ceil_div(tiles, splits);
+    pl.n_splits = (int)ceil_div(tiles, pl.split_tiles);
+    const int64_t grid = ceil_div(pl.items, w / pl.kw) * pl.n_splits * p->pages.n_kv_heads;
+    if (grid > 0x7FFFFFFF || rows * group > 0x7FFFFFFF || ceil_div(rows * p->n_q_heads, MERGE_THREADS / 64) > 0x7FFFFFFF) return false;
+    pl.grid = (unsigned)grid;
+    return true;
+}
+int64_t part_values(const tq_paged_attn_params *p, const Plan &pl) { return pl.n_splits > 1 ? p->rows * p->n_q_heads * (int64_t)pl.n_splits : 0; }
+
+int check_pages(const tq_pages *p, int64_t rows, const char *who) {
+    REQUIRE(p, TQ_ERR_ARG, "%s: null pages", who);
+    REQUIRE(p->batch >= 0 && p->n_kv_heads >= 1 && p->n_pages >= 0 && p->max_blocks >= 0 && rows >= 0, TQ_ERR_ARG, "%s: negative size", who);
+    REQUIRE(p->n_kv_heads <= 65536, TQ_ERR_UNSUPPORTED, "%s: over 65536 KV heads", who);
+    REQUIRE(p->max_blocks < (1 << 24) && rows <= 0x7FFFFFFF, TQ_ERR_UNSUPPORTED, "%s: positions and rows have to fit 32 bits", who);
+    REQUIRE(p->table_stride >= p->max_blocks || p->batch <= 1, TQ_ERR_ARG, "%s: table_stride %lld is under max_blocks %d", who,
+            (long long)p->table_stride, p->max_blocks);
+    REQUIRE(p->cu_new || rows >= p->batch, TQ_ERR_ARG, "%s: %lld rows for %d sequences", who, (long long)rows, p->batch);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p->block_table) | reinterpret_cast<uintptr_t>(p->cu_new) | reinterpret_cast<uintptr_t>(p->lens);
+    REQUIRE(at % 4 == 0, TQ_ERR_ALIGN, "%s: a table is not aligned to its type", who);
+    if (p->batch == 0 || rows == 0) return TQ_OK;
+    REQUIRE(p->lens && (p->block_table || p->max_blocks == 0), TQ_ERR_ARG, "%s: null table", who);
+    return TQ_OK;
+}
+int check_sides(const tq_handle *hk, const tq_handle *hv, const char *who) {
+    const int rc = hk ? check_fast(hk, who) : TQ_OK;
+    return rc ? rc : hv ? check_fast(hv, who) : TQ_OK;
+}
+int check_attn(const tq_paged_attn_params *p) {
+    REQUIRE(p, TQ_ERR_ARG, "tq_paged_attention: null parameters");
+    const int rc = check_pages(&p->pages, p->rows, "tq_paged_attention");
+    if (rc) return rc;
+    REQUIRE(p->n_q_heads >= 1 && p->n_q_heads % p->pages.n_kv_heads == 0, TQ_ERR_ARG,
+            "tq_paged_attention: %d query heads are not a multiple of the KV head count (%d)", p->n_q_heads, p->pages.n_kv_heads);
+    REQUIRE(p->scale > 1e-18f && p->scale < 1e18f, TQ_ERR_ARG, "tq_paged_attention: scale %g is not positive and finite", (double)p->scale);
+    REQUIRE(p->dtype == TQ_F16 || p->dtype == TQ_BF16, TQ_ERR_ARG, "tq_paged_attention: dtype %d is neither float16 nor bfloat16", p->dtype);
+    REQUIRE(p->max_context >= 0 && p->max_new >= 0, TQ_ERR_ARG, "tq_paged_attention: negative size");
+    return TQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tq_append_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *pages, const void *k, const void *v, int64_t rows,
+                    int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, int in_dtype, void *k_pages, void *v_pages,
+                    uint32_t *overrun_dev, void *stream) {
+    int rc = check_sides(hk, hv, "tq_append_paged");
+    rc = rc ? rc : check_pages(pages, rows, "tq_append_paged");
+    if (rc) return rc;
+    REQUIRE(in_dtype == TQ_F16 || in_dtype == TQ_BF16 || in_dtype == TQ_F32, TQ_ERR_ARG, "tq_append_paged: dtype %d is none of float16, bfloat16, float32",
+            in_dtype);
+    if (pages->batch == 0 || rows == 0) return TQ_OK;
+    REQUIRE(k && v && ((k_pages && v_pages) || pages->n_pages == 0), TQ_ERR_ARG, "tq_append_paged: null pointer");
+    const int each = in_dtype == TQ_F32 ? 4 : 2;
+    auto steps_ok = [&](const void *x, int64_t token, int64_t head) { return aligned16(x) && token * each % 16 == 0 && head * each % 16 == 0; };
+    REQUIRE((!hk || steps_ok(k, k_token, k_head)) && (!hv || steps_ok(v, v_token, v_head)) && aligned16(k_pages) && aligned16(v_pages) &&
+                reinterpret_cast<uintptr_t>(k) % each == 0 && reinterpret_cast<uintptr_t>(v) % each == 0,
+            TQ_ERR_ALIGN, "tq_append_paged: pages, and rows and strides of turbo formats, must be multiples of 16 bytes");
+    REQUIRE((reinterpret_cast<uintptr_t>(overrun_dev) & 3u) == 0, TQ_ERR_ALIGN, "tq_append_paged: overrun_dev must be 4-byte aligned");
+    return tqk_append_paged(hk, hv, pages, k, v, rows, k_token, k_head, v_token, v_head, in_dtype, k_pages, v_pages, overrun_dev, (hipStream_t)stream);
+}
+
+int tq_load_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *pages, const void *k_pages, const void *v_pages, int64_t rows,
+                  void *out_k, void *out_v, void *stream) {
+    int rc = check_sides(hk, hv, "tq_load_paged");
+    rc = rc ? rc : check_pages(pages, rows, "tq_load_paged");
+    if (rc) return rc;
+    if (pages->batch == 0 || rows == 0) return TQ_OK;
+    REQUIRE(out_k && out_v && ((k_pages && v_pages) || pages->n_pages == 0), TQ_ERR_ARG, "tq_load_paged: null pointer");
+    REQUIRE(aligned16(out_k) && aligned16(out_v) && aligned16(k_pages) && aligned16(v_pages), TQ_ERR_ALIGN,
+            "tq_load_paged: pages and outputs must be 16-byte aligned");
+    return tqk_load_paged(hk, hv, pages, k_pages, v_pages, rows, out_k, out_v, (hipStream_t)stream);
+}
+
+int64_t tq_paged_attn_workspace_bytes(const tq_paged_attn_params *p) {
+    if (check_attn(p)) return -1;
+    Plan pl;
+    if (p->pages.batch == 0 || p->rows == 0) return 16;
+    if (!make_plan(p, pl)) {
+        tq_set_error("tq_paged_attention: %lld rows are more than a launch takes", (long long)p->rows);
+        return -1;
+    }
+    return part_values(p, pl) * 130 * 4 + 16;
+}
+
+int tq_paged_attention(const tq_handle *hk, const tq_handle *hv, const tq_paged_attn_params *p, const void *q, const void *k_pages,
+                       const void *v_pages, void *out, void *workspace, int64_t workspace_bytes, void *stream) {
+    int rc = check_sides(hk, hv, "tq_paged_attention");
+    rc = rc ? rc : check_attn(p);
+    if (rc) return rc;
+    if (p->pages.batch == 0 || p->rows == 0) return TQ_OK;
+    const bool no_pages = p->pages.n_pages == 0 || p->pages.max_blocks == 0;
+    REQUIRE(q && out && workspace && (no_pages || (k_pages && v_pages)), TQ_ERR_ARG, "tq_paged_attention: null pointer");
+    REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace) && aligned16(k_pages) && aligned16(v_pages) && p->q_token % 8 == 0 && p->q_head % 8 == 0,
+            TQ_ERR_ALIGN, "tq_paged_attention: q, its strides, out, pages and workspace must be multiples of 16 bytes");
+    Plan pl;
+    if (!make_plan(p, pl)) {
+        tq_set_error("tq_paged_attention: %lld rows are more than a launch takes", (long long)p->rows);
+        return TQ_ERR_UNSUPPORTED;
+    }
+    REQUIRE(workspace_bytes >= part_values(p, pl) * 130 * 4 + 16, TQ_ERR_ARG, "tq_paged_attention: the workspace holds %lld bytes, %lld are needed",
+            (long long)workspace_bytes, (long long)(part_values(p, pl) * 130 * 4 + 16));
+    PagedAttnArgs a{};
+    a.r = PagedRows{p->pages, p->rows, tqd::make_fast_div((uint32_t)p->pages.n_kv_heads)};
+    a.q = q; a.out = out; a.q_token = p->q_token; a.q_head = p->q_head;
+    a.bf16 = p->dtype == TQ_BF16; a.causal = p->causal != 0;
+    a.max_context = no_pages ? 0 : pl.max_context;   // nothing is read then
+    a.max_new = pl.max_new;
+    a.group = p->n_q_heads / p->pages.n_kv_heads;
+    a.group_div = tqd::make_fast_div((uint32_t)a.group); a.heads_div = a.r.heads_div;
+    a.k = (const uint8_t *)k_pages; a.v = (const uint8_t *)v_pages;
+    a.scale = p->scale * 1.4426950408889634f;
+    a.v_unscale = 1.0f;
+    if (hk) { a.klut = hk->scaled_lut; a.ks1 = hk->s1_32; a.ks2 = hk->s2_32; a.scale /= hk->value_scale; }
+    if (hv) { a.vlut = hv->scaled_lut; a.vs1 = hv->s1_32; a.vs2 = hv->s2_32; a.v_unscale = 1.0f / hv->value_scale; }
+    a.n_splits = pl.n_splits; a.split_tiles = pl.split_tiles; a.kw = pl.kw;
+    a.part_o = (float *)workspace;
+    a.part_ml = a.part_o + part_values(p, pl) * 128;
+    const int kb = hk ? hk->bits : 8, vb = hv ? hv->bits : 8;
+    const bool share = hk && hv && kb == vb && std::memcmp(hk->centroids_host, hv->centroids_host, sizeof(double) << kb) == 0;
+    hipStream_t s = (hipStream_t)stream;
+    switch (kb) {
+    case 2: rc = tqk_paged_attn_k2(a, vb, share, pl.rb, pl.grid, s); break;
+    case 3: rc = tqk_paged_attn_k3(a, vb, share, pl.rb, pl.grid, s); break;
+    case 4: rc = tqk_paged_attn_k4(a, vb, share, pl.rb, pl.grid, s); break;
+    default: rc = tqk_paged_attn_k8(a, vb, share, pl.rb, pl.grid, s); break;
+    }
+    if (rc || pl.n_splits == 1) return rc;
+    k_paged_merge<<<(unsigned)ceil_div(p->rows * p->n_q_heads, MERGE_THREADS / 64), MERGE_THREADS, 0, s>>>(a);
+    return tq_check_launch("paged_merge");
+}
+
+}  // extern "C"

@@ -30,6 +30,8 @@ struct tq_handle {
     double *projrot64_t;   // [128*128] entry [k*128+j] = (S R^T)[j][k]   (d == 128, WHT, projection)
     void *pair_lut;        // [4^bits] half2: (c[lo], c[hi]) for a pair code (bits <= 3), or [256] for 4
     uint32_t pair_lut_host[256];  // host copy of pair_lut (two handles with equal tables can share one LDS copy)
+    uint32_t *scaled_lut;  // pair_lut of the codebook times value_scale, a factor for which fp16 holds all of it closely
+    float value_scale;
     uint16_t *qjl_frag;    // [3][4][8][64][8] fp16: 64 (S R^T) split into three fp16 terms, as B operands of 16x16x32 matrix instructions (QJL store)
     float qjl_tau;         // first pass (fp16 matrix cores): |value| below qjl_tau * |scaled residual| goes to the second pass
     double qjl_tau2;       // second pass (float64 against the three terms): |value| below qjl_tau2 * |residual| goes to the float64 matrix
@@ -109,6 +111,12 @@ int tqk_q8_0_append(const void *x, int64_t n_seqs, int64_t pos, int64_t n_new, i
                     void *packed, hipStream_t s, const int64_t *pos_dev = nullptr, uint32_t *overrun = nullptr);
 int tqk_q8_0_store_v(const void *x, int64_t n_seqs, int64_t tokens, int in_dtype, void *packed, hipStream_t s);
 int tqk_q8_0_unpack(const void *packed, int64_t n_seqs, int64_t tokens, int8_t *q, float *scales, int kind, hipStream_t s);
+
+int tqk_append_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *p, const void *k, const void *v, int64_t rows, int64_t k_token,
+                     int64_t k_head, int64_t v_token, int64_t v_head, int in_dtype, void *k_pages, void *v_pages, uint32_t *overrun,
+                     hipStream_t s);
+int tqk_load_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *p, const void *k_pages, const void *v_pages, int64_t rows,
+                   void *out_k, void *out_v, hipStream_t s);
 
 int64_t tqk_attn_workspace_bytes(const tq_attn_params *p);
 void tqk_attn_plan(const tq_attn_params *p, int kb, int vb, bool share, bool dense, int64_t ws_bytes, tq_attn_plan *out);

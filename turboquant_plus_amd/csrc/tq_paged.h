@@ -1,0 +1,71 @@
+// Which sequence, block or rows a workgroup has in a launch over a paged cache.
+#pragma once
+#include "tq_internal.h"
+#include "tq_layout.h"
+
+struct PagedRows {
+    tq_pages p;
+    int64_t rows;           // of the new tokens' tensors
+    tqd::FastDiv heads_div; // division by n_kv_heads
+};
+
+struct PagedSeq {
+    int64_t row0;   // its first row in the new tokens' tensors
+    int n;          // its rows; 0 where the tables give rows outside of the tensors
+    int64_t start;  // lens[b]
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedRows &r, int b) {
+    PagedSeq q;
+    const int32_t lo = r.p.cu_new ? r.p.cu_new[b] : b, hi = r.p.cu_new ? r.p.cu_new[b + 1] : b + 1;
+    q.row0 = lo;
+    q.n = lo >= 0 && hi > lo && hi <= r.rows ? hi - lo : 0;
+    q.start = r.p.lens[b];
+    return q;
+}
+// whether an append at lens[b] has a place for the sequence's rows
+__device__ __forceinline__ bool paged_room(const PagedRows &r, const PagedSeq &q) {
+    return q.start >= 0 && q.start + q.n <= (int64_t)r.p.max_blocks * TQ_ROWS_PER_BLOCK;
+}
+// blocks that hold rows of sequence b
+__device__ __forceinline__ int paged_blocks(const PagedRows &r, int b) {
+    const PagedSeq q = paged_seq(r, b);
+    if (q.n == 0 || !paged_room(r, q)) return 0;
+    return (int)((q.start + q.n - 1) / TQ_ROWS_PER_BLOCK - q.start / TQ_ROWS_PER_BLOCK) + 1;
+}
+// One workgroup's look at every sequence: why an append leaves some out.
+__device__ __forceinline__ void paged_report(const PagedRows &r, uint32_t *overrun) {
+    for (int b = threadIdx.x; b < r.p.batch; b += blockDim.x) {
+        const PagedSeq q = paged_seq(r, b);
+        const int32_t lo = r.p.cu_new ? r.p.cu_new[b] : b, hi = r.p.cu_new ? r.p.cu_new[b + 1] : b + 1;
+        uint32_t why = 0;
+        if (q.n == 0) why = lo == hi && lo >= 0 && hi <= r.rows ? 0u : TQ_OVERRUN_NO_PAGE;
+        else if (q.start < 0) why = TQ_OVERRUN_NEGATIVE;
+        else if (!paged_room(r, q)) why = TQ_OVERRUN_NO_ROOM;
+        if (why) atomicOr(overrun, why);
+    }
+}
+
+// Item `item` of the sequences' items laid end to end, count(b) of them to sequence b: its sequence and its number there, the
+// same in every lane; false behind the last one.  Every wavefront of a workgroup calls it and works it out for itself: 64
+// sequences at a time, a sum over the lanes.
+template <class Count> __device__ __forceinline__ bool paged_item(const PagedRows &r, int item, Count count, int &b, int &nth) {
+    const int lane = (int)(threadIdx.x & 63);
+    for (int b0 = 0; b0 < r.p.batch; b0 += 64) {
+        const int c = b0 + lane < r.p.batch ? count(b0 + lane) : 0;
+        int upto = c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int below = __shfl_up(upto, o);
+            if (lane >= o) upto += below;
+        }
+        const unsigned long long behind = __builtin_amdgcn_ballot_w64(upto > item);
+        if (behind) {
+            const int at = __builtin_ctzll(behind);
+            b = b0 + at;
+            nth = item - __builtin_amdgcn_readlane(upto - c, at);
+            return true;
+        }
+        item -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}

@@ -19,6 +19,7 @@
 
 #include "tq_device.h"
 #include "tq_device64.h"
+#include "tq_paged.h"
 
 namespace {
 
@@ -48,6 +49,16 @@ template <> __device__ inline void load8<double>(const double *p, float (&v)[8])
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)p[i];
 }
+template <> __device__ inline void load8<__bf16>(const __bf16 *p, float (&v)[8]) {
+    const uint4 u = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+
 template <typename T> __device__ inline void store8(T *p, const float (&v)[8]);
 template <> __device__ inline void store8<__half>(__half *p, const float (&v)[8]) {
     uint32_t w[4];
@@ -2020,28 +2031,16 @@ struct AppendUnitArgs {
 // TI = float: fp32 rows as three fp16 terms per value, or in the store's two.  Three hold all 24 bits of values above about 2^-10
 // of the row's norm and the others to 2^-34 of it (a row is scaled to a norm of 512 to 1024, where an fp16 term ends at 2^-24):
 // less than the 32-bit sums round.
-template <int BITS, int KIND, bool AS_STORE, typename TI>
-__device__ __forceinline__ void append_units(const TI *x, uint8_t *packed, const AppendUnitArgs &a, const unsigned wg) {
-    constexpr bool F32 = sizeof(TI) == 4;
+// A wavefront's 16 tokens of one block: n_old .. n_end - 1 of its rows are new, row(t) is the input of row t.
+template <int BITS, int KIND, bool AS_STORE, typename TI, class Row>
+__device__ __forceinline__ void append_unit_rows(const Row row, uint8_t *block, const int n_old, const int n_end, const AppendUnitArgs &a) {
+    constexpr bool F32 = !std::is_same<TI, __half>::value, BF16 = F32 && sizeof(TI) == 2;  // bf16 rows go as fp32
     constexpr int NX = F32 ? 8 : 4;  // 16-byte pieces of a lane's 32 inputs
     constexpr int NT = 1 << (BITS - 1);
     constexpr LevelLut LUT = AS_STORE ? LUT_SEARCH : LUT_NONE;
     const int lane = threadIdx.x & 63, n16 = lane & 15, kq = lane >> 4;
     const int unit = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t0 = 16 * unit;
-    const uint32_t seq = a.touched_div.div(wg), nth = wg - seq * a.n_touched;
-    int64_t pos = a.pos, first_block = a.first_block;
-    if (a.pos_dev) {  // the position is read when the launch runs (see resolve_append)
-        pos = *a.pos_dev;
-        if (!append_position_ok(pos, a.n_new, a.capacity, a.overrun, wg == 0)) return;
-        first_block = pos / TQ_ROWS_PER_BLOCK;
-        if ((int64_t)nth >= (pos + a.n_new - 1) / TQ_ROWS_PER_BLOCK - first_block + 1) return;
-    }
-    const int64_t bis = first_block + nth, tok0 = bis * TQ_ROWS_PER_BLOCK;
-    const int n_old = (int)(pos - tok0 < 0 ? 0 : pos - tok0);
-    const int n_end = (int)(pos + a.n_new - tok0 > TQ_ROWS_PER_BLOCK ? TQ_ROWS_PER_BLOCK : pos + a.n_new - tok0);
     if (t0 + 16 <= n_old) return;  // nothing but tokens that stay
-    uint8_t *block = packed + ((int64_t)seq * a.blocks_per_seq + bis) * block_bytes(BITS);
-
     __half *norms = reinterpret_cast<__half *>(block + block_code_bytes(BITS));
     if (t0 >= n_end) {  // nothing but rows past the new ones: norm 0 and the code of 0.0, which is as many dwords in K rows as in V's
         const uint32_t code = a.thr[0] < 0.0f ? 1u << (BITS - 1) : (1u << (BITS - 1)) - 1u;
@@ -2055,11 +2054,19 @@ __device__ __forceinline__ void append_units(const TI *x, uint8_t *packed, const
     }
 
     const int t = t0 + n16;  // the token of this lane's inputs; tokens outside the new ones request a new one's and drop them
-    const TI *row = x + ((int64_t)seq * a.n_new + (tok0 + min(max(t, n_old), n_end - 1) - pos)) * 128;
-    const uint4 *p = reinterpret_cast<const uint4 *>(row + (KIND == TQ_KIND_K ? 32 : 8) * kq);
+    const uint4 *p = reinterpret_cast<const uint4 *>(row(min(max(t, n_old), n_end - 1)) + (KIND == TQ_KIND_K ? 32 : 8) * kq);
     uint4 xb[NX];
+    if constexpr (BF16) {
 #pragma unroll
-    for (int i = 0; i < NX; ++i) xb[i] = p[KIND == TQ_KIND_K ? i : F32 ? 8 * (i >> 1) + (i & 1) : 4 * i];
+        for (int i = 0; i < 4; ++i) {
+            const uint4 h = p[KIND == TQ_KIND_K ? i : 4 * i];
+            xb[2 * i] = make_uint4(h.x << 16, h.x & 0xFFFF0000u, h.y << 16, h.y & 0xFFFF0000u);
+            xb[2 * i + 1] = make_uint4(h.z << 16, h.z & 0xFFFF0000u, h.w << 16, h.w & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NX; ++i) xb[i] = p[KIND == TQ_KIND_K ? i : F32 ? 8 * (i >> 1) + (i & 1) : 4 * i];
+    }
     // V: dword `jd` of the lane's rows 16 dd + n16 of the tile is what the lane stores
     const int jd = BITS == 2 ? kq >> 1 : kq;
     const bool stores = BITS == 4 || (BITS == 3 ? kq < 3 : (kq & 1) == 0);
@@ -2206,6 +2213,24 @@ __device__ __forceinline__ void append_units(const TI *x, uint8_t *packed, const
         const int tn = t0 + 4 * kq + n16;
         if (n16 < 4 && tn >= n_old) norms[tn] = __float2half_rn(gn);
     }
+}
+
+template <int BITS, int KIND, bool AS_STORE, typename TI>
+__device__ __forceinline__ void append_units(const TI *x, uint8_t *packed, const AppendUnitArgs &a, const unsigned wg) {
+    const uint32_t seq = a.touched_div.div(wg), nth = wg - seq * a.n_touched;
+    int64_t pos = a.pos, first_block = a.first_block;
+    if (a.pos_dev) {  // the position is read when the launch runs (see resolve_append)
+        pos = *a.pos_dev;
+        if (!append_position_ok(pos, a.n_new, a.capacity, a.overrun, wg == 0)) return;
+        first_block = pos / TQ_ROWS_PER_BLOCK;
+        if ((int64_t)nth >= (pos + a.n_new - 1) / TQ_ROWS_PER_BLOCK - first_block + 1) return;
+    }
+    const int64_t bis = first_block + nth, tok0 = bis * TQ_ROWS_PER_BLOCK;
+    const int n_old = (int)(pos - tok0 < 0 ? 0 : pos - tok0);
+    const int n_end = (int)(pos + a.n_new - tok0 > TQ_ROWS_PER_BLOCK ? TQ_ROWS_PER_BLOCK : pos + a.n_new - tok0);
+    uint8_t *block = packed + ((int64_t)seq * a.blocks_per_seq + bis) * block_bytes(BITS);
+    append_unit_rows<BITS, KIND, AS_STORE, TI>([&](int t) { return x + ((int64_t)seq * a.n_new + (tok0 + t - pos)) * 128; }, block, n_old,
+                                               n_end, a);
 }
 
 template <int BITS, int KIND, typename TI>
@@ -3113,32 +3138,19 @@ __device__ __forceinline__ int round_half_away(float t) {
 #pragma clang fp contract(off)
     return (int)(t + copysignf(0.49999997f, t));
 }
-template <typename TI, int KIND>
-__device__ __forceinline__ void q8_0_append_block(const TI *x, uint8_t *packed, const Q8AppendArgs &a, const unsigned wg) {
+template <typename TI, int KIND, class Row>
+__device__ __forceinline__ void q8_0_append_rows(const Row row, uint8_t *block, const int n_old, const int n_end, const bool wide) {
     __shared__ __attribute__((aligned(16))) uint8_t rows_s[TQ_ROWS_PER_BLOCK * Q8A_ROW];
     __shared__ __attribute__((aligned(16))) __half scales_s[TQ_ROWS_PER_BLOCK * 4];  // K: [token][group], V: as stored
-    int64_t pos = a.pos, first_block = a.first_block;
-    const uint32_t seq_n = a.touched_div.div(wg), nth = wg - seq_n * a.n_touched;
-    if (a.pos_dev) {  // the position is read when the launch runs (see resolve_append)
-        pos = *a.pos_dev;
-        if (!append_position_ok(pos, a.n_new, a.capacity, a.overrun, wg == 0)) return;
-        first_block = pos / TQ_ROWS_PER_BLOCK;
-        if ((int64_t)nth >= (pos + a.n_new - 1) / TQ_ROWS_PER_BLOCK - first_block + 1) return;
-    }
     const int tid = threadIdx.x;
-    const int64_t seq = seq_n, bis = first_block + nth;
-    const int64_t tok0 = bis * TQ_ROWS_PER_BLOCK;
-    uint8_t *block = packed + (seq * a.blocks_per_seq + bis) * (int64_t)(TQ_ROWS_PER_BLOCK * 136);
-    const int n_old = (int)(pos - tok0 < 0 ? 0 : pos - tok0);
-    const int n_end = (int)(pos + a.n_new - tok0 > TQ_ROWS_PER_BLOCK ? TQ_ROWS_PER_BLOCK : pos + a.n_new - tok0);
     constexpr int NP = TQ_ROWS_PER_BLOCK * 16 / Q8A_THREADS;
     const int c8 = tid & 15;  // the lane's dims: 8 c8 .. 8 c8 + 7
     float v[NP][8];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int t = min(max(i * (Q8A_THREADS / 16) + (tid >> 4), n_old), n_end - 1);  // others request a new row and drop it
-        const TI *p = x + (seq * a.n_new + (tok0 + t - pos)) * 128 + 8 * c8;
-        if (a.wide) {
+        const TI *p = row(t) + 8 * c8;
+        if (wide) {
             load8(p, v[i]);
         } else {
 #pragma unroll
@@ -3200,6 +3212,24 @@ __device__ __forceinline__ void q8_0_append_block(const TI *x, uint8_t *packed, 
 }
 
 template <typename TI, int KIND>
+__device__ __forceinline__ void q8_0_append_block(const TI *x, uint8_t *packed, const Q8AppendArgs &a, const unsigned wg) {
+    int64_t pos = a.pos, first_block = a.first_block;
+    const uint32_t seq_n = a.touched_div.div(wg), nth = wg - seq_n * a.n_touched;
+    if (a.pos_dev) {  // the position is read when the launch runs (see resolve_append)
+        pos = *a.pos_dev;
+        if (!append_position_ok(pos, a.n_new, a.capacity, a.overrun, wg == 0)) return;
+        first_block = pos / TQ_ROWS_PER_BLOCK;
+        if ((int64_t)nth >= (pos + a.n_new - 1) / TQ_ROWS_PER_BLOCK - first_block + 1) return;
+    }
+    const int64_t seq = seq_n, bis = first_block + nth;
+    const int64_t tok0 = bis * TQ_ROWS_PER_BLOCK;
+    uint8_t *block = packed + (seq * a.blocks_per_seq + bis) * (int64_t)(TQ_ROWS_PER_BLOCK * 136);
+    const int n_old = (int)(pos - tok0 < 0 ? 0 : pos - tok0);
+    const int n_end = (int)(pos + a.n_new - tok0 > TQ_ROWS_PER_BLOCK ? TQ_ROWS_PER_BLOCK : pos + a.n_new - tok0);
+    q8_0_append_rows<TI, KIND>([&](int t) { return x + (seq * a.n_new + (tok0 + t - pos)) * 128; }, block, n_old, n_end, a.wide != 0);
+}
+
+template <typename TI, int KIND>
 __global__ __launch_bounds__(Q8A_THREADS) void k_q8_0_append(const TI *x, uint8_t *packed, Q8AppendArgs a) {
     q8_0_append_block<TI, KIND>(x, packed, a, blockIdx.x);
 }
@@ -3242,6 +3272,199 @@ __global__ __launch_bounds__(256) void k_q8_0_unpack(const uint8_t *packed, int8
         scales[(seq * tokens + tok0 + t) * 4 + (e & 3)] =
             __half2float(reinterpret_cast<const __half *>(block + 8 * 2048)[kind == TQ_KIND_V ? q8v_scale(t, e & 3) : e]);
     }
+}
+
+// ---- caches in pages -----------------------------------------------------------------------------------
+// Rows of several sequences, token-major, appended to pages: a workgroup per touched block and side, on the code of the
+// contiguous appends (append_unit_rows, q8_0_append_rows), so the bytes are theirs.  Which sequence and block a workgroup has, it
+// finds by itself from the sequences' lengths in device memory (paged_item), so the grid is only an upper bound.
+// Bound by vector instructions, as the contiguous appends are.
+template <typename TI>
+__global__ __launch_bounds__(APPEND_THREADS, (std::is_same<TI, __half>::value ? 4 : 3)) void k_append_paged(PagedRows r, const TI *xk, const TI *xv, uint8_t *pk,
+                                                                               uint8_t *pv, int64_t k_token, int64_t k_head, int64_t v_token,
+                                                                               int64_t v_head, int kb, int vb, int k_wide, int v_wide,
+                                                                               AppendUnitArgs ka, AppendUnitArgs va, uint32_t *overrun) {
+    const unsigned half = gridDim.x >> 1;
+    const bool is_v = blockIdx.x >= half;
+    const unsigned wg = is_v ? blockIdx.x - half : blockIdx.x;
+    const uint32_t item = r.heads_div.div(wg), head = wg - item * r.heads_div.d;
+    if (overrun && blockIdx.x == 0) paged_report(r, overrun);
+    int b, nth;
+    if (!paged_item(r, (int)item, [&](int s) { return paged_blocks(r, s); }, b, nth)) return;
+    const PagedSeq q = paged_seq(r, b);
+    const int64_t bis = q.start / TQ_ROWS_PER_BLOCK + nth, tok0 = bis * TQ_ROWS_PER_BLOCK;
+    const int n_old = (int)(q.start - tok0 < 0 ? 0 : q.start - tok0);
+    const int n_end = (int)(q.start + q.n - tok0 > TQ_ROWS_PER_BLOCK ? TQ_ROWS_PER_BLOCK : q.start + q.n - tok0);
+    const int page = __builtin_amdgcn_readfirstlane(r.p.block_table[b * r.p.table_stride + bis]);
+    if (page < 0 || page >= r.p.n_pages) {
+        if (overrun && threadIdx.x == 0 && !is_v && head == 0) atomicOr(overrun, TQ_OVERRUN_NO_PAGE);
+        return;
+    }
+    const int64_t at = (int64_t)page * r.p.n_kv_heads + head;
+    const TI *x = is_v ? xv + head * v_head : xk + head * k_head;
+    const int64_t step = is_v ? v_token : k_token;
+    x += (q.row0 + (tok0 - q.start)) * step;
+    auto row = [&](int t) { return x + t * step; };
+    if (!is_v) {
+        switch (kb) {
+        case 2: append_unit_rows<2, TQ_KIND_K, false, TI>(row, pk + at * block_bytes(2), n_old, n_end, ka); break;
+        case 3: append_unit_rows<3, TQ_KIND_K, false, TI>(row, pk + at * block_bytes(3), n_old, n_end, ka); break;
+        case 4: append_unit_rows<4, TQ_KIND_K, false, TI>(row, pk + at * block_bytes(4), n_old, n_end, ka); break;
+        default: q8_0_append_rows<TI, TQ_KIND_K>(row, pk + at * (TQ_ROWS_PER_BLOCK * 136), n_old, n_end, k_wide != 0); break;
+        }
+    } else {
+        switch (vb) {
+        case 2: append_unit_rows<2, TQ_KIND_V, false, TI>(row, pv + at * block_bytes(2), n_old, n_end, va); break;
+        case 3: append_unit_rows<3, TQ_KIND_V, false, TI>(row, pv + at * block_bytes(3), n_old, n_end, va); break;
+        case 4: append_unit_rows<4, TQ_KIND_V, false, TI>(row, pv + at * block_bytes(4), n_old, n_end, va); break;
+        default: q8_0_append_rows<TI, TQ_KIND_V>(row, pv + at * (TQ_ROWS_PER_BLOCK * 136), n_old, n_end, v_wide != 0); break;
+        }
+    }
+}
+
+// Positions of several sequences back as fp16 rows: a workgroup per 64-token tile and side, a wavefront per 16 tokens.
+// K codes are a lane's own dwords (as in load_k16_body), V codes are gathered from the tile in LDS (load_v16_body); eight matrix
+// instructions with the +-1 operand turn 16 tokens back, and whole rows leave through LDS.  The codebook enters as fp16 multiples
+// (tq_handle::scaled_lut), the norms in 32 bits.
+struct PagedLoadSide {
+    const uint8_t *pages;
+    __half *out;
+    const uint4 *afrag;
+    const float *s1;
+    const uint32_t *lut;
+    float unscale;   // 1 / value_scale
+    int bits;        // 8: q8_0-style rows
+};
+template <int BITS, int KIND>
+__device__ __forceinline__ void load_paged_tile(const PagedLoadSide &a, const uint8_t *block, const int half, const int lo, const int hi,
+                                                __half *out, const int64_t step, uint32_t *lut_s, uint8_t *tile_s, uint8_t *xpose_s) {
+    // rows lo .. hi - 1 of the tile are wanted; row t of it goes to out + t * step
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n16 = lane & 15, kc = lane >> 4;
+    constexpr int XROW = LOAD16_XROW, PIECES = BITS * 64 + 8;
+    for (int e = tid; e < (1 << (2 * BITS)); e += 256) lut_s[e] = a.lut[e];
+    half8_t af[8];
+#pragma unroll
+    for (int f = 0; f < 8; ++f) af[f] = __builtin_bit_cast(half8_t, a.afrag[f * 64 + lane]);
+    uint32_t smask[16];
+#pragma unroll
+    for (int w = 0; w < 16; ++w)
+        smask[w] = (a.s1[32 * kc + 2 * w] < 0.0f ? 0x8000u : 0u) | (a.s1[32 * kc + 2 * w + 1] < 0.0f ? 0x80000000u : 0u);
+    const __half *norms = reinterpret_cast<const __half *>(block + block_code_bytes(BITS)) + 64 * half;
+    // K: token 16 wave + n16; V: the tokens of which a wavefront's codes lie in the same dword of a row (load_v16_body)
+    const int tl = KIND == TQ_KIND_K ? 16 * wave + n16 : 16 * (n16 >> 2) + 4 * wave + (n16 & 3);
+    const float g = __half2float(norms[tl]) * a.unscale;
+    uint32_t cw[BITS];
+    if constexpr (KIND == TQ_KIND_K) {
+#pragma unroll
+        for (int j = 0; j < BITS; ++j) cw[j] = *reinterpret_cast<const uint32_t *>(block + j * 2048 + (64 * half + tl) * 16 + kc * 4);
+    } else {
+        for (int e = tid; e < PIECES - 8; e += 256)
+            reinterpret_cast<uint4 *>(tile_s)[e] = *reinterpret_cast<const uint4 *>(block + (e >> 6) * 2048 + (64 * half + (e & 63)) * 16);
+    }
+    __syncthreads();
+    uint4 xb[4];
+    if constexpr (KIND == TQ_KIND_K) {
+        uint32_t tail = 0;
+        if constexpr (BITS == 3) tail = (cw[0] >> 24) | ((cw[1] >> 24) << 8) | ((cw[2] >> 24) << 16);
+        const char *lut = reinterpret_cast<const char *>(lut_s);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            xb[ks].x = *reinterpret_cast<const uint32_t *>(lut + group_pair_offset<BITS>(cw, tail, 4 * ks));
+            xb[ks].y = *reinterpret_cast<const uint32_t *>(lut + group_pair_offset<BITS>(cw, tail, 4 * ks + 1));
+            xb[ks].z = *reinterpret_cast<const uint32_t *>(lut + group_pair_offset<BITS>(cw, tail, 4 * ks + 2));
+            xb[ks].w = *reinterpret_cast<const uint32_t *>(lut + group_pair_offset<BITS>(cw, tail, 4 * ks + 3));
+        }
+    } else {
+        const int hf = kc >> 1, r0 = 32 * (kc & 1);
+        const int p = ((tl & 60) | (hf << 1)) | ((tl >> 1) & 1), grp = p >> 4, k = p & 15, hs = (tl & 1) * BITS;
+        constexpr uint32_t CM = (1u << BITS) - 1u;
+        uint32_t hv[32];
+        if (BITS == 3 && wave == 3) {
+            const int sh = 6 * (k - 12) + hs;
+#pragma unroll
+            for (int v = 0; v < 32; ++v) {
+                const uint8_t *rowp = tile_s + (r0 + v) * 16 + grp * 4;
+                const uint32_t tail = (*reinterpret_cast<const uint32_t *>(rowp) >> 24) |
+                                      ((*reinterpret_cast<const uint32_t *>(rowp + 1024) >> 24) << 8) |
+                                      ((*reinterpret_cast<const uint32_t *>(rowp + 2048) >> 24) << 16);
+                hv[v] = lut_s[(tail >> sh) & CM] & 0xFFFFu;
+            }
+        } else {
+            const int dw = k / tqd::pairs_per_dword(BITS), sh = 2 * BITS * (k % tqd::pairs_per_dword(BITS)) + hs;
+            const uint8_t *col = tile_s + dw * 1024 + grp * 4;
+#pragma unroll
+            for (int v = 0; v < 32; ++v) hv[v] = lut_s[(*reinterpret_cast<const uint32_t *>(col + (r0 + v) * 16) >> sh) & CM] & 0xFFFFu;
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+            xb[ks] = make_uint4(hv[8 * ks] | (hv[8 * ks + 1] << 16), hv[8 * ks + 2] | (hv[8 * ks + 3] << 16), hv[8 * ks + 4] | (hv[8 * ks + 5] << 16),
+                                hv[8 * ks + 6] | (hv[8 * ks + 7] << 16));
+    }
+    uint32_t o[16];
+    unrotate_unit16(af, xb, g, smask, o);
+    uint8_t *mine = xpose_s + wave * (16 * XROW);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4 *>(mine + n16 * XROW + kc * 64 + c * 16) = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const int t = KIND == TQ_KIND_K ? 16 * wave + 4 * c + (lane >> 4) : 16 * c + 4 * wave + (lane >> 4);
+        const uint4 piece = *reinterpret_cast<const uint4 *>(mine + (4 * c + (lane >> 4)) * XROW + (lane & 15) * 16);
+        if (t >= lo && t < hi) stream_store<STREAM_LOAD_OUT>(reinterpret_cast<uint4 *>(out + t * step + 8 * (lane & 15)), piece);
+    }
+}
+// 8-bit rows: a thread takes 8 values of a token
+template <int KIND>
+__device__ __forceinline__ void load_paged_tile_q8(const uint8_t *block, const int half, const int lo, const int hi, __half *out, const int64_t step) {
+    const __half *scales = reinterpret_cast<const __half *>(block + 8 * 2048);
+    for (int e = threadIdx.x; e < 64 * 16; e += 256) {
+        // lanes: K rows 8-byte pieces of a row, V rows the tokens of a dim's 16 bytes
+        const int t = KIND == TQ_KIND_K ? e >> 4 : (e >> 8) * 16 + (e & 15), c8 = KIND == TQ_KIND_K ? e & 15 : (e >> 4) & 15;
+        if (t < lo || t >= hi) continue;
+        const float d = __half2float(scales[KIND == TQ_KIND_V ? q8v_scale(64 * half + t, c8 >> 2) : (64 * half + t) * 4 + (c8 >> 2)]);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int dim = 8 * c8 + j;
+            v[j] = d * (float)(int8_t)block[KIND == TQ_KIND_V ? q8v_byte(64 * half + t, dim) : (dim >> 4) * 2048 + (64 * half + t) * 16 + (dim & 15)];
+        }
+        store8(out + t * step + 8 * c8, v);
+    }
+}
+__global__ __launch_bounds__(256) void k_load_paged(PagedRows r, PagedLoadSide ks, PagedLoadSide vs) {
+    __shared__ uint32_t lut_s[256];
+    __shared__ __attribute__((aligned(16))) uint8_t tile_s[4 * 64 * 16];
+    __shared__ __attribute__((aligned(16))) uint8_t xpose_s[LOAD16_XPOSE_BYTES];
+    const unsigned side = gridDim.x >> 1;
+    const bool is_v = blockIdx.x >= side;
+    const unsigned wg = is_v ? blockIdx.x - side : blockIdx.x;
+    const uint32_t item = r.heads_div.div(wg), head = wg - item * r.heads_div.d;
+    int b, nth;
+    if (!paged_item(r, (int)item >> 1, [&](int s) { return paged_blocks(r, s); }, b, nth)) return;
+    const PagedSeq q = paged_seq(r, b);
+    const int64_t bis = q.start / TQ_ROWS_PER_BLOCK + nth;
+    const int half = (int)(item & 1);
+    const int64_t tok0 = bis * TQ_ROWS_PER_BLOCK + 64 * half;
+    const int lo = (int)(q.start - tok0 < 0 ? 0 : q.start - tok0 > 64 ? 64 : q.start - tok0);
+    const int hi = (int)(q.start + q.n - tok0 > 64 ? 64 : q.start + q.n - tok0);
+    if (lo >= hi) return;
+    const int page = __builtin_amdgcn_readfirstlane(r.p.block_table[b * r.p.table_stride + bis]);
+    if (page < 0 || page >= r.p.n_pages) return;
+    const int64_t at = (int64_t)page * r.p.n_kv_heads + head, step = (int64_t)r.p.n_kv_heads * 128;
+    const PagedLoadSide &a = is_v ? vs : ks;
+    __half *out = a.out + (q.row0 + (tok0 - q.start)) * step + head * 128;
+#define TQ_LOAD_PAGED(B)                                                                                                              if (is_v) load_paged_tile<B, TQ_KIND_V>(vs, vs.pages + at * block_bytes(B), half, lo, hi, out, step, lut_s, tile_s, xpose_s);      else load_paged_tile<B, TQ_KIND_K>(ks, ks.pages + at * block_bytes(B), half, lo, hi, out, step, lut_s, tile_s, xpose_s)
+    switch (a.bits) {
+    case 2: TQ_LOAD_PAGED(2); break;
+    case 3: TQ_LOAD_PAGED(3); break;
+    case 4: TQ_LOAD_PAGED(4); break;
+    default:
+        if (is_v) load_paged_tile_q8<TQ_KIND_V>(vs.pages + at * (TQ_ROWS_PER_BLOCK * 136), half, lo, hi, out, step);
+        else load_paged_tile_q8<TQ_KIND_K>(ks.pages + at * (TQ_ROWS_PER_BLOCK * 136), half, lo, hi, out, step);
+    }
+#undef TQ_LOAD_PAGED
 }
 
 #define DISPATCH_T(dt, NAME, F)                      \
@@ -4702,6 +4925,65 @@ int tqk_load_kv(const tq_handle *hk, const tq_handle *hv, const void *packed_k, 
 #undef TQ_LKV_V
 #undef TQ_LKV
     return tq_check_launch("load_kv16");
+}
+
+// blocks of all sequences' new rows at the worst alignment, an upper bound known without the lengths
+static int64_t paged_blocks_bound(const tq_pages *p, int64_t rows) {
+    if (!p->cu_new) return p->batch;
+    return std::min<int64_t>(rows, rows / TQ_ROWS_PER_BLOCK + 2 * (int64_t)p->batch);
+}
+
+int tqk_append_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *p, const void *k, const void *v, int64_t rows, int64_t k_token,
+                     int64_t k_head, int64_t v_token, int64_t v_head, int in_dtype, void *k_pages, void *v_pages, uint32_t *overrun,
+                     hipStream_t s) {
+    for (const tq_handle *h : {hk, hv})
+        if (h && !append_units_ok(h, TQ_F16)) {
+            tq_set_error("tq_append_paged: the codebook is not symmetric, which the matrix-core append needs");
+            return TQ_ERR_UNSUPPORTED;
+        }
+    const int64_t grid = 2 * paged_blocks_bound(p, rows) * p->n_kv_heads;
+    if (grid == 0) return TQ_OK;
+    if (grid > 0x7FFFFFFF) {
+        tq_set_error("tq_append_paged: %lld rows of %d heads are more than a launch takes", (long long)rows, p->n_kv_heads);
+        return TQ_ERR_UNSUPPORTED;
+    }
+    AppendUnitArgs ka{}, va{};
+    if (hk) ka = make_append_unit_args(hk, 0, nullptr, 1, TQ_ROWS_PER_BLOCK, nullptr);
+    if (hv) va = make_append_unit_args(hv, 0, nullptr, 1, TQ_ROWS_PER_BLOCK, nullptr);
+    const PagedRows r{*p, rows, make_fast_div((uint32_t)p->n_kv_heads)};
+    const int each = in_dtype == TQ_F32 ? 4 : 2;
+    auto wide = [&](const void *x, int64_t token, int64_t head) {
+        return (int)(reinterpret_cast<uintptr_t>(x) % 16 == 0 && token * each % 16 == 0 && head * each % 16 == 0);
+    };
+#define TQ_APPEND_PAGED(T)                                                                                                                    k_append_paged<T><<<(unsigned)grid, APPEND_THREADS, 0, s>>>(r, (const T *)k, (const T *)v, (uint8_t *)k_pages, (uint8_t *)v_pages, k_token,                                                                 k_head, v_token, v_head, hk ? hk->bits : 0, hv ? hv->bits : 0,                                                                             wide(k, k_token, k_head), wide(v, v_token, v_head), ka, va, overrun)
+    if (in_dtype == TQ_F16) TQ_APPEND_PAGED(__half);
+    else if (in_dtype == TQ_BF16) TQ_APPEND_PAGED(__bf16);
+    else TQ_APPEND_PAGED(float);
+#undef TQ_APPEND_PAGED
+    return tq_check_launch("append_paged");
+}
+
+int tqk_load_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *p, const void *k_pages, const void *v_pages, int64_t rows,
+                   void *out_k, void *out_v, hipStream_t s) {
+    const int64_t grid = 4 * paged_blocks_bound(p, rows) * p->n_kv_heads;
+    if (grid == 0) return TQ_OK;
+    if (grid > 0x7FFFFFFF) {
+        tq_set_error("tq_load_paged: %lld rows of %d heads are more than a launch takes", (long long)rows, p->n_kv_heads);
+        return TQ_ERR_UNSUPPORTED;
+    }
+    auto side = [](const tq_handle *h, const void *pages, void *out) {
+        PagedLoadSide a{};
+        a.pages = (const uint8_t *)pages;
+        a.out = (__half *)out;
+        a.bits = 8;
+        if (h) {
+            a.afrag = (const uint4 *)h->rfrag16k_inv; a.s1 = h->s1_32; a.lut = h->scaled_lut; a.unscale = 1.0f / h->value_scale; a.bits = h->bits;
+        }
+        return a;
+    };
+    k_load_paged<<<(unsigned)grid, 256, 0, s>>>(PagedRows{*p, rows, make_fast_div((uint32_t)p->n_kv_heads)}, side(hk, k_pages, out_k),
+                                                 side(hv, v_pages, out_v));
+    return tq_check_launch("load_paged");
 }
 
 int tqk_load(const tq_handle *h, const void *packed, int64_t n_seqs, int64_t tokens, int kind, void *out,

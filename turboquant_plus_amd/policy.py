@@ -20,6 +20,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 from . import _lib as L
+from .paged import PagedAttention, append_paged, load_paged, new_pages
 from .turbo import DecodeAttention, TurboCodec, append_layer, packed_bytes, q8_0_append, q8_0_store, store_layer
 
 FORMATS = ("q8_0", "turbo4", "turbo3", "turbo2")
@@ -154,3 +155,17 @@ class LayerKV:
 
     def attention(self, batch: int, n_q_heads: int, n_kv_heads: int, tokens: int, **kw) -> DecodeAttention:
         return DecodeAttention(self.k_codec, self.v_codec, batch, n_q_heads, n_kv_heads, tokens, **kw)
+
+    # ---- the layer's cache in pages (paged.py) ------------------------------------------------------------------
+    def new_pages(self, n_pages: int, n_kv_heads: int):
+        """Zeroed (k_pages, v_pages) for append_paged()."""
+        return new_pages(self.k_codec, self.v_codec, n_pages, n_kv_heads)
+
+    def append_paged(self, k, v, k_pages, v_pages, block_table, starts, cu_new=None, *, overrun=None):
+        return append_paged(self.k_codec, self.v_codec, k, v, k_pages, v_pages, block_table, starts, cu_new, overrun=overrun)
+
+    def load_paged(self, k_pages, v_pages, block_table, starts, cu_new=None, rows: int | None = None, *, out=None):
+        return load_paged(self.k_codec, self.v_codec, k_pages, v_pages, block_table, starts, cu_new, rows, out=out)
+
+    def paged_attention(self, n_q_heads: int, n_kv_heads: int, **kw) -> PagedAttention:
+        return PagedAttention(self.k_codec, self.v_codec, n_q_heads, n_kv_heads, **kw)
