@@ -78,16 +78,18 @@ def attend64(lay, q, kp, vp, table, lens, new, causal, scale=D ** -0.5):
         if lay.k_codec is not None:
             x = x @ rotation(lay.k_codec).T
         seen = tt.arange(c, device="cuda")[None] < (c - n + tt.arange(n, device="cuda")[:, None] + 1 if causal else c)
+        seen = seen.expand(n, c).repeat_interleave(g, 0)
         for h in range(hkv):
             kk, vv = k[pages, h].reshape(-1, D)[:c], v[pages, h].reshape(-1, D)[:c]
-            for j in range(h * g, (h + 1) * g):
-                logits = scale * x[:, j] @ kk.T
-                w = tt.softmax(tt.where(seen, logits, -float("inf")), -1).nan_to_num(0.0) if c else tt.zeros((n, 0), device="cuda").double()
-                y = w @ vv
-                off = 2 ** -11 * (1 + scale * (x[:, j].square() @ kk.square().T).sqrt())
-                size = vv.norm(dim=-1)
-                tol[at:at + n, j] = (eps / 2 + 2 ** -10) * y.norm(dim=-1) + 4 * (w * size * off).norm(dim=-1) + 2 ** -20 * (w @ size) + 2.0 ** -24
-                out[at:at + n, j] = y if lay.v_codec is None else y @ rotation(lay.v_codec)
+            xx = x[:, h * g:(h + 1) * g].reshape(-1, D)
+            logits = scale * xx @ kk.T
+            w = tt.softmax(tt.where(seen, logits, -float("inf")), -1).nan_to_num(0.0) if c else tt.zeros((n * g, 0), device="cuda").double()
+            y = w @ vv
+            off = 2 ** -11 * (1 + scale * (xx.square() @ kk.square().T).sqrt())
+            size = vv.norm(dim=-1)
+            tol[at:at + n, h * g:(h + 1) * g] = ((eps / 2 + 2 ** -10) * y.norm(dim=-1) + 4 * (w * size * off).norm(dim=-1) + 2 ** -20 * (w @ size)
+                                                 + 2.0 ** -24).view(n, g)
+            out[at:at + n, h * g:(h + 1) * g] = (y if lay.v_codec is None else y @ rotation(lay.v_codec)).view(n, g, D)
         at += n
     return out, tol
 
@@ -316,6 +318,88 @@ def test_a_query_that_is_no_number_stays_in_its_row():
     assert not same[3, 2] and not same[9, 0] and int(same.sum()) == 78
     big = (q * 0).nan_to_num(0.0).bfloat16() + 3e30      # a row's size is taken out before fp16
     assert tt.isfinite(lay.paged_attention(4, 1, scale=1e-17)(big, kp, vp, table, ints(lens), cumulative([20]))).all()
+
+
+@pytest.mark.parametrize("kf,vf", [("turbo3", "turbo3"), ("turbo4", "turbo4"), ("q8_0", "turbo2"), ("turbo2", "q8_0")])
+@pytest.mark.parametrize("hq,new,lens", [(4, 1, 500), (8, 1, 5000), (4, 3, 5000), (4, 7, 400), (4, 10, 5000), (4, 40, 300)])
+def test_few_rows_that_are_no_numbers_or_huge(kf, vf, hq, new, lens):
+    """The same at every number of rows: one and several passes, 28, 40 and 160 rows, joined through memory and not."""
+    lay, lens = layer(kf, vf), (lens, 200)
+    kp, vp, table = filled(lay, lens, 1, 24)
+    gen = tt.Generator("cuda").manual_seed(25)
+    q = tt.randn((2 * new, hq, D), generator=gen, device="cuda").half()
+    args = kp, vp, table, ints(lens), cumulative([new, new])
+    want = lay.paged_attention(hq, 1)(q, *args)
+    bad = q.clone()
+    bad[0, 1, 17], bad[-1, 3, 5] = float("nan"), float("-inf")
+    got = lay.paged_attention(hq, 1)(bad, *args)
+    same = (got == want).all(-1)
+    assert not tt.isfinite(got[0, 1]).any() and int(same.sum()) >= 2 * new * hq - 2
+    if kf != "q8_0":     # a rotated row holds its infinity in every place
+        assert not tt.isfinite(got[-1, 3]).any()
+    # a row's size is taken out before fp16, and logits that 32 bits hold with steps of many units have a softmax all the same
+    for factor, scale in ((1e30, 1e-17), (1e-30, 1e17), (3e20, 1.0)):
+        x = (q.float() * factor).bfloat16()
+        y, tol = attend64(lay, x, kp, vp, table, lens, [new, new], True, scale)
+        out = lay.paged_attention(hq, 1, scale=scale)(x, *args)
+        assert tt.isfinite(out).all()
+        if factor < 1:
+            check(out, y, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,batch,new,top", [(32, 8, 64, 1, 260), (64, 8, 64, 1, 260), (8, 2, 300, 1, 130), (4, 1, 520, 2, 70), (32, 8, 32, 1, 3000), (64, 8, 16, 2, 3100),
+                                                  (2, 2, 5, 1, 9000), (12, 1, 3, 1, 20000)])
+@pytest.mark.parametrize("kf,vf,dtype", [("turbo3", "turbo3", "fp16"), ("turbo4", "turbo4", "bf16"), ("turbo4", "turbo3", "fp16"), ("q8_0", "q8_0", "fp16")])
+def test_few_rows_of_ragged_batches(kf, vf, dtype, hq, hkv, batch, new, top):
+    """Groups that share a workgroup, sequences shorter than a workgroup's part, empty ones, ones without rows, many parts."""
+    lay = layer(kf, vf)
+    rng = np.random.default_rng(26)
+    lens = [int(top if b == batch - 1 else 0 if b % 17 == 3 else rng.integers(1, top + 1)) for b in range(batch)]
+    news = [0 if b % 13 == 5 else int(rng.integers(1, new + 1)) for b in range(batch)]
+    kp, vp, table = filled(lay, lens, hkv, 27)
+    gen = tt.Generator("cuda").manual_seed(28)
+    q = tt.randn((sum(news) + 1, hq, D), generator=gen, device="cuda").to(DTYPES[dtype])
+    out = tt.full_like(q, 7.0)
+    attn = lay.paged_attention(hq, hkv)
+    attn(q, kp, vp, table, ints(lens), cumulative(news), max_new=new, out=out)
+    assert (out[-1] == 7).all()
+    want, tol = attend64(lay, q[:-1], kp, vp, table, lens, news, True)
+    check(out[:-1], want, tol)
+    again = tt.full_like(q, 7.0)
+    attn(q, kp, vp, table, ints(lens), cumulative(news), max_new=new, max_context=top + 1000, out=again)     # another split of the positions
+    check(again[:-1], want, tol)
+
+
+def test_two_captured_steps_of_different_plans_share_a_workspace():
+    """Replayed in turn, with eager work between: each finds its counters whatever the other left in them."""
+    lay = layer("turbo4", "turbo4")
+    lens = (9000, 300, 5000)
+    kp, vp, table = filled(lay, lens, 2, 29)
+    gen = tt.Generator("cuda").manual_seed(30)
+    q = tt.randn((6, 8, D), generator=gen, device="cuda").half()
+    attn = lay.paged_attention(8, 2)
+    calls = [lambda out: attn(q[:3], kp, vp, table, ints_lens, max_context=9000, out=out),
+             lambda out: attn(q, kp, vp, table, ints_lens, cu, max_context=20000, max_new=2, out=out)]
+    ints_lens, cu = ints(lens), cumulative([2, 2, 2])
+    outs = [tt.empty((n, 8, D), dtype=tt.float16, device="cuda") for n in (3, 6)]
+    want = [call(tt.empty_like(out)) for call, out in zip(calls, outs)]
+    graphs = []
+    side = tt.cuda.Stream()
+    with tt.cuda.stream(side):
+        for call, out in zip(calls, outs):
+            call(out)
+            side.synchronize()
+            g = tt.cuda.CUDAGraph()
+            with tt.cuda.graph(g, stream=side):
+                call(out)
+            graphs.append(g)
+    tt.cuda.synchronize()
+    for turn in (0, 1, 0, 0, 1, 1, 0):
+        outs[turn].fill_(7.0)
+        graphs[turn].replay()
+        tt.cuda.synchronize()
+        assert tt.equal(outs[turn], want[turn]), turn
+        assert tt.equal(calls[1 - turn](tt.empty_like(outs[1 - turn])), want[1 - turn])
 
 
 @pytest.mark.parametrize("causal", [True, False])

@@ -60,6 +60,12 @@ unsigned long long next_nonce() {
     return (z >> 40) ? z : z | (1ull << 63);  // the upper 24 bits tag the Sparse-V words and must not be zero
 }
 
+}  // namespace
+
+unsigned long long tqk_attn_nonce() { return next_nonce(); }
+
+namespace {
+
 struct WsLayout {
     int64_t part_o, part_ml, skip_slots, flags, pass_totals, total;
 };

@@ -155,10 +155,11 @@ __device__ __forceinline__ float half_at(uint2 u, int i) {
 // NH: query heads per pass.  SHARE: K and V decode through one table (same width, same centroids).  LIST: the call carries
 // a sparse logit bias (eight heads).  Work distribution, progress marks and the merge are those of k_decode_attn: a workgroup of W
 // wavefronts owns W consecutive splits of one group (or a.gpw groups of fewer splits each).
-template <int KBITS, int VBITS, bool SPARSE, bool SHARE, int NH, bool LIST>
+template <int KBITS, int VBITS, bool SPARSE, bool SHARE, int NH, bool LIST, bool PAGED = false>
 __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs a) {
     static_assert(NH == 4 ? !LIST : NH == 8, "query heads per pass");
     static_assert(!SHARE || KBITS == VBITS, "a shared table needs equal code widths");
+    static_assert(!PAGED || (!SPARSE && !LIST), "what a paged step has");
     constexpr int HG = NH / 4, U = NH / 4;
     constexpr int KBLOCK = TQ_ROWS_PER_BLOCK * (16 * KBITS + 2), VBLOCK = TQ_ROWS_PER_BLOCK * (16 * VBITS + 2);
     constexpr int LUT_TOTAL = table_bytes(KBITS) + (SHARE ? 0 : table_bytes(VBITS));
@@ -174,6 +175,7 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
     constexpr uint32_t V_HIGH = KBITS == 4 && VBITS == 4 && !SHARE ? 65536u : 0u;
     const char *const klut_s = smem + K_AT, *const vlut_s = smem + V_AT;
 
+    __shared__ float row_scale[PAGED ? 64 : 1];   // PAGED: [group of the workgroup][head], a query row's power of two and the logit scale
     const int tid = threadIdx.x, lane = tid & 63;
     const int n = lane & 15, q4 = lane >> 4, h = lane & (NH - 1), r = n / NH;
     const uint32_t kown = 4u * lane, vown = kown + V_HIGH;   // 4-bit codes: this lane's copy
@@ -183,9 +185,10 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
     const int wave_g = a.gpw > 1 ? (wave & (gw - 1)) : wave, wave0 = wave - wave_g;
     const int gidx = a.gpw > 1 ? (wave >> a.gw_shift) : 0;
     const int tid_g = tid - 64 * wave0;
-    const int wgs_per_group = a.wgs_per_group;
-    const int group = __builtin_amdgcn_readfirstlane(a.gpw > 1 ? (int)blockIdx.x * a.gpw + gidx : (int)(blockIdx.x / wgs_per_group));
-    const int part = a.gpw > 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(blockIdx.x % wgs_per_group));
+    const int places = a.wgs_per_group;   // partials that a group has room for
+    int wgs_per_group = places;
+    const int group = __builtin_amdgcn_readfirstlane(a.gpw > 1 ? (int)blockIdx.x * a.gpw + gidx : (int)(blockIdx.x / places));
+    const int part = a.gpw > 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(blockIdx.x % places));
     const int pass_y = HG == 2 ? (int)blockIdx.y : 0;   // one set of four heads is always one pass
     const int head_off = a.head_off + pass_y * a.pass_heads, pgroup = pass_y * a.n_groups + group;
     const int split = part * n_waves + wave_g;
@@ -200,8 +203,16 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
         n_tiles = (tokens_now + 63) >> 6;
         tiles_per_split = (n_tiles + a.n_splits - 1) / a.n_splits;
     }
-    const int t_begin = split * tiles_per_split;
-    const int t_end = min(t_begin + tiles_per_split, n_tiles);
+    PagedPass pg{};
+    int paged_begin = 0, paged_end = 0;
+    if constexpr (PAGED) {
+        pg = paged_pass(a, group, head_off, NH);
+        tokens_now = pg.most;
+        n_tiles = (tokens_now + 63) >> 6;
+        if (!paged_tiles(a, pg, n_tiles, part, wave_g, wgs_per_group, paged_begin, paged_end)) return;
+    }
+    const int t_begin = PAGED ? paged_begin : split * tiles_per_split;
+    const int t_end = PAGED ? paged_end : min(t_begin + tiles_per_split, n_tiles);
     // first of this lane's four tokens of its u-th step (tile-relative)
     int t4[U];
 #pragma unroll
@@ -209,6 +220,16 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
 
     const uint8_t *kbase = a.k + (int64_t)group * a.blocks_per_seq * KBLOCK;
     const uint8_t *vbase = a.v + (int64_t)group * a.blocks_per_seq * VBLOCK;
+    // the block of a tile: of the sequence's own, or (PAGED) of its page, whose number is looked up two tiles ahead
+    auto page_of = [&](int tile) { return PAGED ? scalar_entry(pg.table, __builtin_amdgcn_readfirstlane(tile >> 1)) : 0; };
+    auto is_page = [&](int page) { return page >= 0 && page < a.pg.r.p.n_pages; };
+    auto block_no = [&](int tile, int page) -> int64_t {
+        return PAGED ? (int64_t)(is_page(page) ? page : 0) * a.pg.r.p.n_kv_heads + pg.kvh : (int64_t)(tile >> 1);
+    };
+    if constexpr (PAGED) {
+        kbase = a.k;
+        vbase = a.v;
+    }
     // The first tile's rows are requested before anything else, so that the table build and the query rotation overlap
     // the first trip to memory; afterwards one tile ahead into the same registers, the norms with them.  Row n of step j is
     // token 4 quad_of(j, n / 4) + n % 4: the steps differ by constants.  After the split's last tile the prefetch has every
@@ -217,22 +238,22 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
     const uint32_t voff = VBITS == 4 ? 16u * n + 2048u * q4 : 16u * lane;
     constexpr int KPD = parts_dwords(KBITS, false), VPD = parts_dwords(VBITS, true);
     uint32_t kw[4][KPD], vw[4][VPD];
-    auto load_k = [&](int tile, bool any) {
-        const uint8_t *p = kbase + (int64_t)(tile >> 1) * KBLOCK + (any ? (tile & 1) * 1024 : 0);
+    auto load_k = [&](int tile, int page, bool any) {
+        const uint8_t *p = kbase + block_no(tile, page) * KBLOCK + (any ? (tile & 1) * 1024 : 0);
         load_parts<KBITS, VBITS>(p, any ? koff : 0u, kw);
     };
-    auto load_v = [&](int tile, bool any) {
-        const uint8_t *p = vbase + (int64_t)(tile >> 1) * VBLOCK + (any ? (tile & 1) * 1024 : 0);
+    auto load_v = [&](int tile, int page, bool any) {
+        const uint8_t *p = vbase + block_no(tile, page) * VBLOCK + (any ? (tile & 1) * 1024 : 0);
         load_parts<VBITS, 4>(p, any ? voff : 0u, vw);   // row 16 j + n
     };
     auto load_norms = [&](const uint8_t *block_norms, int tile, uint2 (&g)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) g[u] = *reinterpret_cast<const uint2 *>(block_norms + (tile & 1) * 128 + 2u * (uint32_t)t4[u]);
     };
-    auto k_norms = [&](int tile) { return kbase + (int64_t)(tile >> 1) * KBLOCK + TQ_ROWS_PER_BLOCK * 16 * KBITS; };
-    auto v_norms = [&](int tile) { return vbase + (int64_t)(tile >> 1) * VBLOCK + TQ_ROWS_PER_BLOCK * 16 * VBITS; };
+    auto k_norms = [&](int tile, int page) { return kbase + block_no(tile, page) * KBLOCK + TQ_ROWS_PER_BLOCK * 16 * KBITS; };
+    auto v_norms = [&](int tile, int page) { return vbase + block_no(tile, page) * VBLOCK + TQ_ROWS_PER_BLOCK * 16 * VBITS; };
     unsigned long long arrivals_seen = 0ull;
-    if (wgs_per_group > 1 && tid == 0) arrivals_seen = ld_dev(arrival_counter(a, pgroup, wgs_per_group));
+    if (wgs_per_group > 1 && tid == 0) arrivals_seen = ld_dev(arrival_counter(a, pgroup, PAGED ? PAGED_COUNTER_STEP : places));
     // pair-table entries for the table build
     uint4 kpair = make_uint4(0u, 0u, 0u, 0u), vpair = kpair;
     if constexpr (KBITS == 3) kpair.x = a.klut[lane];
@@ -243,11 +264,14 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
 #pragma unroll
     for (int u = 0; u < U; ++u) gk[u] = gv[u] = make_uint2(0u, 0u);
     int tile = t_begin;
+    int page = 0, page_n = 0;    // PAGED: of this tile and the next
     if (tile < t_end) {
-        load_k(tile, true);
-        load_norms(k_norms(tile), tile, gk);
-        load_v(tile, true);
-        load_norms(v_norms(tile), tile, gv);
+        page = page_of(tile);
+        page_n = page_of(min(tile + 1, t_end - 1));
+        load_k(tile, page, true);
+        load_norms(k_norms(tile, page), tile, gk);
+        load_v(tile, page, true);
+        load_norms(v_norms(tile, page), tile, gv);
     }
     if (tid == 0) {
         lead = 0;
@@ -255,6 +279,10 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
     }
 
     auto load_q = [&](int head, float &x0, float &x1) {   // heads past the group's last one repeat it (their results are not written)
+        if constexpr (PAGED) {
+            paged_query(a, pg, head_off + head, lane, x0, x1);
+            return;
+        }
         const int64_t e = ((int64_t)group * a.q_group + min(head_off + head, a.q_group - 1)) * 128 + 2 * lane;
         if (a.q_dtype == TQ_F16) {
             const __half *qp = reinterpret_cast<const __half *>(a.q);
@@ -308,6 +336,13 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
         _Float16 *qw = reinterpret_cast<_Float16 *>(q_stage) + head * 128;
         float x0 = xq0, x1 = xq1;
         if (head != wave_g) load_q(head, x0, x1);
+        if constexpr (PAGED) {
+            float back;
+            const float f = row_exponent(x0, x1, back);
+            x0 *= f;
+            x1 *= f;
+            if (lane == 0) row_scale[gidx * NH + head] = back * a.scale_log2e;
+        }
         if (a.ks1) {
             x0 *= a.ks1[2 * lane];
             x1 *= a.ks1[2 * lane + 1];
@@ -316,10 +351,11 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
             x1 *= a.ks2[2 * lane + 1] * RSQRT128;
         }
         // the rotated query is rounded to fp16 once, with the logit scale (times log2 e) folded in
-        qw[2 * lane] = (_Float16)(x0 * a.scale_log2e);
-        qw[2 * lane + 1] = (_Float16)(x1 * a.scale_log2e);
+        // (PAGED: the scale is with the row's power of two, applied to the logits)
+        qw[2 * lane] = (_Float16)(PAGED ? x0 : x0 * a.scale_log2e);
+        qw[2 * lane + 1] = (_Float16)(PAGED ? x1 : x1 * a.scale_log2e);
     }
-    if (wgs_per_group > 1 && tid == 0) install_tag(a, arrival_counter(a, pgroup, wgs_per_group), arrivals_seen);
+    if (wgs_per_group > 1 && tid == 0) install_tag(a, arrival_counter(a, pgroup, PAGED ? PAGED_COUNTER_STEP : places), arrivals_seen);
     __syncthreads();
     half8_t qb[4];   // B operand of QK: head h, the dims of element t of this quarter
 #pragma unroll
@@ -335,6 +371,9 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
     unsigned nskip = 0;   // Sparse V: skipped (query, position) pairs of this wavefront (wave-uniform)
     bool v_ahead = true;  // Sparse V: this tile's V row was requested while the previous tile was processed
     const unsigned long long head_ok = __builtin_amdgcn_ballot_w64(head_off + h < a.q_group);
+    const float f_row = PAGED ? row_scale[gidx * NH + h] : 1.0f;
+    // PAGED: the positions that this lane's head sees
+    const int lim = PAGED && pg.rows > 0 ? paged_limit(a, pg, min(head_off + h, pg.rows - 1)) : 0;
 #pragma unroll 1
     while (tile < t_end) {
         {   // issue priority = tiles behind the leader (wave-uniform, so the branches are scalar)
@@ -348,8 +387,12 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
         const bool more = tile + 1 < t_end;
         const int tile_n = more ? tile + 1 : tile;
         uint2 gv_next[U];
-        load_norms(v_norms(tile_n), tile_n, gv_next);
+        int page_after = 0;
+        if constexpr (PAGED) page_after = page_of(min(tile + 2, t_end - 1));
+        load_norms(v_norms(tile_n, page_n), tile_n, gv_next);
         const int n_valid = tokens_now - tile * 64;   // >= 64 except in the sequence's last tile
+        const bool masked = PAGED && (pg.least - tile * 64 < 64 || !is_page(page));   // some head does not see all of the tile
+        const int seen = PAGED && is_page(page) ? lim - tile * 64 : 0;                 // positions of it that this lane's head sees
         float bias4[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -419,10 +462,11 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[u][i] = LIST ? fmaf(s[u][i], half_at(gk[u], i), bias4[u][i]) : s[u][i] * half_at(gk[u], i);
-                if (n_valid < 64 && t4[u] + i >= n_valid) s[u][i] = -INFINITY;
+                if constexpr (PAGED) s[u][i] = rounded_product(s[u][i], f_row);
+                if (PAGED ? masked && t4[u] + i >= seen : n_valid < 64 && t4[u] + i >= n_valid) s[u][i] = -INFINITY;
             }
-        load_k(tile_n, more);   // kw is dead now
-        load_norms(k_norms(tile_n), tile_n, gk);
+        load_k(tile_n, page_n, more);   // kw is dead now
+        load_norms(k_norms(tile_n, page_n), tile_n, gk);
 
         // ---- online softmax in base 2; a head's state is the same in all of its lanes ----------------------
         float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
@@ -472,7 +516,7 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
                 v_ahead = false;
                 continue;
             }
-            if (!v_ahead) load_v(tile, true);
+            if (!v_ahead) load_v(tile, page, true);
         }
 
         exchange_parts<VBITS>(vw);
@@ -484,6 +528,12 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
             const half2_t lo = {(_Float16)(p[u][0] * half_at(gv[u], 0)), (_Float16)(p[u][1] * half_at(gv[u], 1))};
             const half2_t hi = {(_Float16)(p[u][2] * half_at(gv[u], 2)), (_Float16)(p[u][3] * half_at(gv[u], 3))};
             w[u] = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+            if constexpr (PAGED) {
+                if (masked) {   // what a masked place holds may be no number
+                    w[u].x &= (t4[u] < seen ? 0xFFFFu : 0u) | (t4[u] + 1 < seen ? 0xFFFF0000u : 0u);
+                    w[u].y &= (t4[u] + 2 < seen ? 0xFFFFu : 0u) | (t4[u] + 3 < seen ? 0xFFFF0000u : 0u);
+                }
+            }
         }
         // copies of four heads hold one step each: the even one takes its neighbour's as well, so that the products are the
         // same ones as with eight heads
@@ -503,11 +553,15 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
                 for (int hf = 0; hf < 2; ++hf)
                     acc_o[c][hf] = mfma16(operand(quad_at<VBITS>(vw[c], vlut_s, vown, 2 * st, hf), quad_at<VBITS>(vw[c], vlut_s, vown, 2 * st + 1, hf)),
                                           pb[st], acc_o[c][hf]);
-        load_v(tile_n, more);
+        load_v(tile_n, page_n, more);
         v_ahead = true;
 #pragma unroll
         for (int u = 0; u < U; ++u) gv[u] = gv_next[u];
         ++tile;
+        if constexpr (PAGED) {
+            page = page_n;
+            page_n = page_after;
+        }
     }
 
     // ---- end of split: the column copies are added, the workgroup's wavefronts merge in LDS and write one partial ------
@@ -531,7 +585,7 @@ __global__ __launch_bounds__(NH == 8 ? 768 : 1024) void k_decode_turbo(AttnArgs 
         }
     if (lane < NH) *reinterpret_cast<float2 *>(mine + 512 + 2 * (h & 3)) = make_float2(m_run, l_tot);
     if (SPARSE && lane == 0 && nskip) atomicAdd(&skipped, nskip);
-    finish_group<HG, SPARSE>(a, slot, group, pgroup, head_off, wgs_per_group, part, tid, tid_g, gw, wave0, reinterpret_cast<float *>(smem), &skipped);
+    finish_group<HG, SPARSE, PAGED>(a, slot, group, pgroup, head_off, wgs_per_group, part, tid, tid_g, gw, wave0, reinterpret_cast<float *>(smem), &skipped);
 }
 
 template <int KB, int VB, bool SHARE> void launch_pair(const AttnArgs &a, int n_heads, bool sparse, dim3 grid, int waves, hipStream_t s) {
@@ -563,6 +617,20 @@ bool tqk_launch_decode_turbo(const AttnArgs &a, int kb, int vb, bool share, int 
         return true;
     }
     TQ_PAIR(4, 4) TQ_PAIR(4, 2) TQ_PAIR(2, 4) TQ_PAIR(3, 4) TQ_PAIR(4, 3)
+#undef TQ_PAIR
+    return false;
+}
+
+bool tqk_launch_paged_turbo(const AttnArgs &a, int kb, int vb, bool share, int n_heads, dim3 grid, int waves, hipStream_t s) {
+    const size_t lds = (size_t)a.gpw * 1024 * (n_heads / 4);
+    const unsigned wg = 64u * (unsigned)waves;
+#define TQ_PAIR(K, V, SH)                                                                                            \
+    if (kb == K && vb == V && share == SH) {                                                                         \
+        if (n_heads == 8) k_decode_turbo<K, V, false, SH, 8, false, true><<<grid, wg, lds, s>>>(a);                  \
+        else k_decode_turbo<K, V, false, SH, 4, false, true><<<grid, wg, lds, s>>>(a);                               \
+        return true;                                                                                                 \
+    }
+    TQ_PAIR(4, 4, true) TQ_PAIR(4, 4, false) TQ_PAIR(4, 2, false) TQ_PAIR(2, 4, false) TQ_PAIR(3, 4, false) TQ_PAIR(4, 3, false)
 #undef TQ_PAIR
     return false;
 }

@@ -3,13 +3,14 @@
 #include <cmath>
 #include <cstring>
 
+#include "tq_attn_rows.h"
 #include "tq_check.h"
 #include "tq_paged_attn.h"
 
-int tqk_paged_attn_k2(const tqpaged::PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s);
-int tqk_paged_attn_k3(const tqpaged::PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s);
-int tqk_paged_attn_k4(const tqpaged::PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s);
-int tqk_paged_attn_k8(const tqpaged::PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s);
+int tqk_paged_attn_k2(const tqpaged::PagedAttnArgs &a, int vb, tqpaged::PagedKind kind, unsigned grid, hipStream_t s);
+int tqk_paged_attn_k3(const tqpaged::PagedAttnArgs &a, int vb, tqpaged::PagedKind kind, unsigned grid, hipStream_t s);
+int tqk_paged_attn_k4(const tqpaged::PagedAttnArgs &a, int vb, tqpaged::PagedKind kind, unsigned grid, hipStream_t s);
+int tqk_paged_attn_k8(const tqpaged::PagedAttnArgs &a, int vb, tqpaged::PagedKind kind, unsigned grid, hipStream_t s);
 
 namespace {
 
@@ -63,28 +64,75 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedAttnArgs a) 
 }
 
 struct Plan {
-    int rb, kw, n_splits, split_tiles, max_context, max_new;
+    PagedKind kind;
+    int kw, n_splits, split_tiles, max_context, max_new;
     int64_t items;   // row blocks of all sequences, an upper bound
     unsigned grid;
+    // few rows: k_decode_attn and k_decode_turbo
+    bool few, lane_tables;
+    int hg, wpw, gpw, parts, passes, wg_tiles, splits;
 };
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-bool make_plan(const tq_paged_attn_params *p, Plan &pl) {
+struct Formats {
+    int kb, vb;    // code widths, 8 for 8-bit rows
+    bool share;    // one codebook
+};
+bool plan_few(const tq_paged_attn_params *p, const Formats &f, int64_t most, Plan &pl) {
+    const bool turbo_k = f.kb != 8, turbo_v = f.vb != 8;
+    pl.hg = most > 4 ? 2 : 1;
+    pl.passes = (int)ceil_div(most, 4 * pl.hg);
+    const int64_t groups = (int64_t)p->pages.batch * p->pages.n_kv_heads, units = groups * pl.passes, tiles = std::max<int64_t>(1, ceil_div(pl.max_context, 64));
+    const int wmax = tqattn::max_waves_per_workgroup(turbo_v ? 0 : 8, pl.hg), resident = pl.hg == 1 && turbo_v ? 16 : 8;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256ll * resident / units, ceil_div(tiles, 2)));
+    pl.gpw = 1;
+    if (want <= wmax / 2) {   // several groups to a workgroup
+        int64_t s = 1;
+        while (2 * s <= want) s *= 2;
+        int64_t g = wmax / s;
+        while (g > 1 && (groups % g != 0 || units / g < 256)) g /= 2;
+        if (g > 1) {
+            pl.gpw = (int)g;
+            pl.wpw = (int)(g * s);
+            pl.splits = (int)s;
+            pl.parts = 1;
+            pl.wg_tiles = (int)tiles;
+        }
+    }
+    if (pl.gpw == 1) {
+        pl.wpw = wmax;
+        if (pl.hg == 2 && turbo_k && turbo_v && want % 12 == 0) pl.wpw = 12;
+        while (pl.wpw > 1 && pl.wpw > want) pl.wpw /= 2;
+        while (pl.wpw > 4 && pl.wpw % 2 == 0 && units * ceil_div(want, pl.wpw) < 256) pl.wpw /= 2;
+        pl.wg_tiles = (int)ceil_div(tiles, ceil_div(want, pl.wpw));
+        pl.parts = (int)ceil_div(tiles, pl.wg_tiles);
+        pl.splits = pl.parts * pl.wpw;
+    }
+    const int tables = tqk_decode_turbo_lds(f.kb, f.vb, f.share) + pl.gpw * 1024 * pl.hg;
+    const int64_t wgs = units * pl.parts / pl.gpw, per_cu = std::min<int64_t>(ceil_div(wgs, 256), std::max(1, (pl.hg == 2 ? 12 : 16) / pl.wpw));
+    pl.lane_tables = turbo_k && turbo_v && (f.kb == 4 || f.vb == 4) && per_cu * tables <= 160 * 1024 && ceil_div(tiles, pl.splits) >= 3 && pl.wpw >= 4;
+    if (wgs / pl.passes > 0x7FFFFFFF || pl.passes > 65535) return false;
+    pl.grid = (unsigned)(wgs / pl.passes);
+    pl.n_splits = 1;
+    return true;
+}
+bool make_plan(const tq_paged_attn_params *p, const Formats &f, Plan &pl) {
     const int64_t group = p->n_q_heads / p->pages.n_kv_heads, rows = p->rows;
     const int64_t max_new = p->pages.cu_new ? (p->max_new > 0 ? std::min<int64_t>(p->max_new, rows) : rows) : 1;
     pl.max_new = (int)max_new;
-    const int64_t most = max_new * group;
-    pl.rb = most <= 16 ? 1 : most <= 32 ? 2 : 4;
-    const int64_t tile = 16 * pl.rb;
-    const int w = paged_waves(pl.rb);
+    const int64_t most = max_new * group, space = (int64_t)p->pages.max_blocks * TQ_ROWS_PER_BLOCK;
+    pl.max_context = (int)(p->max_context > 0 ? std::min<int64_t>(p->max_context, space) : space);
+    pl.few = most <= 16;
+    if (pl.few) return plan_few(p, f, most, pl);
+    pl.kind = most <= 32 ? ROWS_32 : most <= 48 ? ROWS_48 : most < 1024 ? CHUNK_128 : CHUNK_256;
+    const int64_t tile = rows_of(pl.kind);
     pl.items = std::min(p->pages.batch * ceil_div(most, tile), rows * group / tile + p->pages.batch);
-    const int64_t room = (int64_t)p->pages.max_blocks * TQ_ROWS_PER_BLOCK;
-    pl.max_context = (int)(p->max_context > 0 ? std::min<int64_t>(p->max_context, room) : room);
-    const int64_t tiles = std::max<int64_t>(1, ceil_div(pl.max_context, 64));
-    // wavefronts that fill the chip: two per SIMD, four where a wavefront has one block of rows
-    const int64_t want = pl.rb == 1 ? 4096 : 2048, blocks = pl.items * p->pages.n_kv_heads;
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(pl.max_context, 64)), blocks = pl.items * p->pages.n_kv_heads;
+    // wavefronts (chunks: workgroups) that fill the chip, and the least that one is given
+    const int w = pl.kind == ROWS_32 || pl.kind == ROWS_48 ? ROWS_WAVES : 1;   // wavefronts that can share a row block
+    const int64_t want = pl.kind == ROWS_32 ? 2048 : pl.kind == ROWS_48 ? 1024 : pl.kind == CHUNK_128 ? 512 : 256, least = w > 1 ? 2 : 8;
     pl.kw = 1;
     while (pl.kw < w && blocks * pl.kw < want && tiles >= 2 * pl.kw) pl.kw *= 2;
-    int64_t splits = std::max<int64_t>(1, std::min(ceil_div(want, blocks * pl.kw), tiles / (2 * pl.kw)));
+    const int64_t splits = std::max<int64_t>(1, std::min(ceil_div(want, blocks * pl.kw), tiles / (least * pl.kw)));
     pl.split_tiles = (int)ceil_div(tiles, splits);
     pl.n_splits = (int)ceil_div(tiles, pl.split_tiles);
     const int64_t grid = ceil_div(pl.items, w / pl.kw) * pl.n_splits * p->pages.n_kv_heads;
@@ -92,7 +140,61 @@ bool make_plan(const tq_paged_attn_params *p, Plan &pl) {
     pl.grid = (unsigned)grid;
     return true;
 }
-int64_t part_values(const tq_paged_attn_params *p, const Plan &pl) { return pl.n_splits > 1 ? p->rows * p->n_q_heads * (int64_t)pl.n_splits : 0; }
+// partial results, of a row's 128 sums, maximum and sum of weights each
+int64_t part_values(const tq_paged_attn_params *p, const Plan &pl) {
+    // few rows: a partial has places for whole sets of four; one more per group holds its counter of finished workgroups
+    if (pl.few) return pl.parts > 1 ? (int64_t)p->pages.batch * p->pages.n_kv_heads * pl.passes * (pl.parts + 1) * 4 * pl.hg : 0;
+    return pl.n_splits > 1 ? p->rows * p->n_q_heads * (int64_t)pl.n_splits : 0;
+}
+// most bytes that the call needs with any formats
+int64_t workspace_bytes_of(const tq_paged_attn_params *p, bool &ok) {
+    int64_t most = 0;
+    ok = true;
+    for (const Formats &f : {Formats{3, 3, true}, Formats{3, 8, false}, Formats{8, 3, false}}) {
+        Plan pl;
+        ok = ok && make_plan(p, f, pl);
+        if (ok) most = std::max(most, part_values(p, pl));
+    }
+    return most * 130 * 4 + 16;
+}
+int attend_few(const tq_handle *hk, const tq_handle *hv, const tq_paged_attn_params *p, const Plan &pl, const Formats &f, const void *q, const void *k,
+               const void *v, void *out, void *ws, int max_context, hipStream_t s) {
+    const int64_t groups = (int64_t)p->pages.batch * p->pages.n_kv_heads, partials = groups * pl.passes * pl.parts;
+    tqattn::AttnArgs a{};
+    a.q = q; a.k = (const uint8_t *)k; a.v = (const uint8_t *)v; a.out = (float *)out;
+    a.scale_log2e = p->scale * 1.4426950408889634f;
+    a.pg.v_unscale = 1.0f;
+    if (hk) { a.klut = hk->scaled_lut; a.ks1 = hk->s1_32; a.ks2 = hk->s2_32; a.scale_log2e /= hk->value_scale; }
+    if (hv) { a.vlut = hv->scaled_lut; a.vs1 = hv->s1_32; a.vs2 = hv->s2_32; a.pg.v_unscale = 1.0f / hv->value_scale; }
+    a.part_o = (float *)ws;
+    a.part_ml = a.part_o + partials * 4 * pl.hg * 128;
+    a.flags = (unsigned long long *)(a.part_ml + partials * 4 * pl.hg * 2);
+    a.nonce = tqk_attn_nonce();
+    a.n_groups = (int)groups;
+    a.n_splits = pl.splits;
+    a.q_group = pl.max_new * (p->n_q_heads / p->pages.n_kv_heads);
+    a.pass_heads = 4 * pl.hg;
+    a.gpw = pl.gpw;
+    while ((1 << a.gw_shift) < pl.splits) ++a.gw_shift;
+    a.wgs_per_group = pl.parts;
+    a.pg.r = PagedRows{p->pages, p->rows, tqd::make_fast_div((uint32_t)p->pages.n_kv_heads)};
+    a.pg.heads_div = tqd::make_fast_div((uint32_t)(p->n_q_heads / p->pages.n_kv_heads));
+    a.pg.q_token = p->q_token; a.pg.q_head = p->q_head;
+    a.pg.max_context = max_context; a.pg.max_new = pl.max_new;
+    a.pg.causal = p->causal != 0; a.pg.bf16 = p->dtype == TQ_BF16;
+    a.pg.wg_tiles = pl.wg_tiles;
+    a.pg.wg_div = tqd::make_fast_div((uint32_t)pl.wg_tiles);
+    a.pg.wave_div = tqd::make_fast_div((uint32_t)pl.wpw);
+    const dim3 grid(pl.grid, (unsigned)pl.passes);
+    const size_t lds = (size_t)pl.wpw * pl.hg * tqattn::MERGE_FLOATS * sizeof(float) + (size_t)pl.gpw * 1024 * pl.hg;
+    const bool built = pl.lane_tables ? tqk_launch_paged_turbo(a, f.kb, f.vb, f.share, 4 * pl.hg, grid, pl.wpw, s)
+                                      : tqk_launch_paged(a, f.kb, f.vb, f.share, pl.hg, grid, 64u * (unsigned)pl.wpw, lds, s);
+    if (!built) {
+        tq_set_error("tq_paged_attention: K of %d bits with V of %d bits is not built", f.kb, f.vb);
+        return TQ_ERR_UNSUPPORTED;
+    }
+    return tq_check_launch("paged_attention");
+}
 
 int check_pages(const tq_pages *p, int64_t rows, const char *who) {
     REQUIRE(p, TQ_ERR_ARG, "%s: null pages", who);
@@ -161,13 +263,11 @@ int tq_load_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *page
 
 int64_t tq_paged_attn_workspace_bytes(const tq_paged_attn_params *p) {
     if (check_attn(p)) return -1;
-    Plan pl;
     if (p->pages.batch == 0 || p->rows == 0) return 16;
-    if (!make_plan(p, pl)) {
-        tq_set_error("tq_paged_attention: %lld rows are more than a launch takes", (long long)p->rows);
-        return -1;
-    }
-    return part_values(p, pl) * 130 * 4 + 16;
+    bool ok;
+    const int64_t need = workspace_bytes_of(p, ok);
+    if (!ok) tq_set_error("tq_paged_attention: %lld rows are more than a launch takes", (long long)p->rows);
+    return ok ? need : -1;
 }
 
 int tq_paged_attention(const tq_handle *hk, const tq_handle *hv, const tq_paged_attn_params *p, const void *q, const void *k_pages,
@@ -180,19 +280,25 @@ int tq_paged_attention(const tq_handle *hk, const tq_handle *hv, const tq_paged_
     REQUIRE(q && out && workspace && (no_pages || (k_pages && v_pages)), TQ_ERR_ARG, "tq_paged_attention: null pointer");
     REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace) && aligned16(k_pages) && aligned16(v_pages) && p->q_token % 8 == 0 && p->q_head % 8 == 0,
             TQ_ERR_ALIGN, "tq_paged_attention: q, its strides, out, pages and workspace must be multiples of 16 bytes");
+    const int kb = hk ? hk->bits : 8, vb = hv ? hv->bits : 8;
+    const bool share = hk && hv && kb == vb && std::memcmp(hk->centroids_host, hv->centroids_host, sizeof(double) << kb) == 0;
+    bool ok;
+    const int64_t need = workspace_bytes_of(p, ok);
     Plan pl;
-    if (!make_plan(p, pl)) {
+    const Formats f{kb, vb, share};
+    if (!ok || !make_plan(p, f, pl)) {
         tq_set_error("tq_paged_attention: %lld rows are more than a launch takes", (long long)p->rows);
         return TQ_ERR_UNSUPPORTED;
     }
-    REQUIRE(workspace_bytes >= part_values(p, pl) * 130 * 4 + 16, TQ_ERR_ARG, "tq_paged_attention: the workspace holds %lld bytes, %lld are needed",
-            (long long)workspace_bytes, (long long)(part_values(p, pl) * 130 * 4 + 16));
+    REQUIRE(workspace_bytes >= need, TQ_ERR_ARG, "tq_paged_attention: the workspace holds %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+    if (pl.few) return attend_few(hk, hv, p, pl, f, q, k_pages, v_pages, out, workspace, no_pages ? 0 : pl.max_context, (hipStream_t)stream);
     PagedAttnArgs a{};
     a.r = PagedRows{p->pages, p->rows, tqd::make_fast_div((uint32_t)p->pages.n_kv_heads)};
     a.q = q; a.out = out; a.q_token = p->q_token; a.q_head = p->q_head;
     a.bf16 = p->dtype == TQ_BF16; a.causal = p->causal != 0;
     a.max_context = no_pages ? 0 : pl.max_context;   // nothing is read then
     a.max_new = pl.max_new;
+    a.blocks_each = p->pages.cu_new ? 0 : (int)ceil_div(p->n_q_heads / p->pages.n_kv_heads, rows_of(pl.kind));
     a.group = p->n_q_heads / p->pages.n_kv_heads;
     a.group_div = tqd::make_fast_div((uint32_t)a.group); a.heads_div = a.r.heads_div;
     a.k = (const uint8_t *)k_pages; a.v = (const uint8_t *)v_pages;
@@ -203,14 +309,13 @@ int tq_paged_attention(const tq_handle *hk, const tq_handle *hv, const tq_paged_
     a.n_splits = pl.n_splits; a.split_tiles = pl.split_tiles; a.kw = pl.kw;
     a.part_o = (float *)workspace;
     a.part_ml = a.part_o + part_values(p, pl) * 128;
-    const int kb = hk ? hk->bits : 8, vb = hv ? hv->bits : 8;
-    const bool share = hk && hv && kb == vb && std::memcmp(hk->centroids_host, hv->centroids_host, sizeof(double) << kb) == 0;
+    a.share = share;
     hipStream_t s = (hipStream_t)stream;
     switch (kb) {
-    case 2: rc = tqk_paged_attn_k2(a, vb, share, pl.rb, pl.grid, s); break;
-    case 3: rc = tqk_paged_attn_k3(a, vb, share, pl.rb, pl.grid, s); break;
-    case 4: rc = tqk_paged_attn_k4(a, vb, share, pl.rb, pl.grid, s); break;
-    default: rc = tqk_paged_attn_k8(a, vb, share, pl.rb, pl.grid, s); break;
+    case 2: rc = tqk_paged_attn_k2(a, vb, pl.kind, pl.grid, s); break;
+    case 3: rc = tqk_paged_attn_k3(a, vb, pl.kind, pl.grid, s); break;
+    case 4: rc = tqk_paged_attn_k4(a, vb, pl.kind, pl.grid, s); break;
+    default: rc = tqk_paged_attn_k8(a, vb, pl.kind, pl.grid, s); break;
     }
     if (rc || pl.n_splits == 1) return rc;
     k_paged_merge<<<(unsigned)ceil_div(p->rows * p->n_q_heads, MERGE_THREADS / 64), MERGE_THREADS, 0, s>>>(a);

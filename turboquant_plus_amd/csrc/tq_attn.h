@@ -5,6 +5,7 @@
 #include <utility>
 
 #include "tq_device.h"
+#include "tq_paged.h"
 
 namespace tqattn {
 
@@ -150,6 +151,21 @@ __device__ __forceinline__ float max_over_blocks(float v) {
     return v;
 }
 
+// A step over a paged cache (tq_paged_attention): the kernels with PAGED find a group's rows, context and blocks through the
+// tables.  A group's "query heads" are then its new tokens' heads, row t * heads + h, of which each sees positions of its own.
+constexpr int PAGED_COUNTER_STEP = 32;   // words from one group's arrival counter to the next: cache lines of their own
+struct PagedStep {
+    PagedRows r;
+    tqd::FastDiv heads_div;      // division by the query heads per KV head
+    // a workgroup's tiles where a group has one of its own (gpw == 1), the same for long and short sequences, and division by
+    // them and by its wavefronts
+    int wg_tiles;
+    tqd::FastDiv wg_div, wave_div;
+    int64_t q_token, q_head;
+    int max_context, max_new, causal, bf16;
+    float v_unscale;             // 1 / value_scale of V's table
+};
+
 struct AttnArgs {
     const void *q;       // [groups*4][128] queries in the original domain, q_dtype
     int q_dtype;
@@ -185,7 +201,82 @@ struct AttnArgs {
     int wgs_per_group;      // gpw == 1: n_splits / wavefronts per workgroup
     float tau;
     int pass_heads;         // heads per pass; blockIdx.y numbers the passes of a launch, whose partials and counters follow each other
+    PagedStep pg;           // PAGED kernels only
 };
+
+// What a group's pass has in a paged cache
+struct PagedPass {
+    int64_t row0;      // the sequence's first row
+    int kvh, rows;     // KV head; the group's rows
+    int ctx, n;        // tokens, new ones among them
+    int least, most;   // positions that the pass's first and last rows see (0: it has none)
+    const int32_t *table;
+};
+__device__ __forceinline__ int paged_limit(const AttnArgs &a, const PagedPass &g, int row) {
+    const int seen = a.pg.causal ? g.ctx - g.n + (int)a.pg.heads_div.div((uint32_t)row) + 1 : g.ctx;
+    return seen < 0 ? 0 : seen;
+}
+__device__ __forceinline__ PagedPass paged_pass(const AttnArgs &a, int group, int head_off, int heads) {
+    const uint32_t b = a.pg.r.heads_div.div((uint32_t)group);
+    PagedPass g;
+    g.kvh = group - (int)(b * a.pg.r.heads_div.d);
+    const tq_pages &p = a.pg.r.p;
+    const int32_t lo = p.cu_new ? scalar_entry(p.cu_new, b) : (int32_t)b, hi = p.cu_new ? scalar_entry(p.cu_new, b + 1) : (int32_t)b + 1;
+    g.row0 = lo;
+    g.n = lo >= 0 && hi > lo && hi <= a.pg.r.rows ? hi - lo : 0;
+    g.rows = min(g.n, a.pg.max_new) * (int)a.pg.heads_div.d;
+    g.ctx = min(max(scalar_entry(p.lens, b), 0), a.pg.max_context);
+    const bool some = head_off < g.rows;
+    g.least = some ? paged_limit(a, g, head_off) : 0;
+    g.most = some ? paged_limit(a, g, min(head_off + heads, g.rows) - 1) : 0;
+    g.table = p.block_table + b * p.table_stride;
+    return g;
+}
+// Tiles [begin, end) of a wavefront, and in how many workgroups the group's tiles are; false: this workgroup has none of them.
+// Workgroups hold equal numbers of tiles: those behind a short sequence's end leave at once, and a ragged batch's long sequences
+// have no more to a wavefront than the others.
+__device__ __forceinline__ bool paged_tiles(const AttnArgs &a, const PagedPass &g, int n_tiles, int part, int wave_g, int &parts, int &begin, int &end) {
+    if (a.gpw > 1) {   // several groups in the workgroup: each has all of its wavefronts there
+        const int per = (n_tiles + a.n_splits - 1) >> a.gw_shift;
+        parts = 1;
+        begin = wave_g * per;
+        end = min(begin + per, n_tiles);
+        return true;
+    }
+    parts = max(1, (int)a.pg.wg_div.div((uint32_t)(n_tiles + a.pg.wg_tiles - 1)));
+    if (part >= parts) return false;
+    const int first = part * a.pg.wg_tiles, here = min(n_tiles - first, a.pg.wg_tiles);
+    const int per = (int)a.pg.wave_div.div((uint32_t)(here + (int)a.pg.wave_div.d - 1));
+    begin = first + wave_g * per;
+    end = min(begin + per, first + here);
+    return true;
+}
+// a power of two that brings a row's largest value to 1 .. 2, so that fp16 holds the row whatever its size; and its inverse
+__device__ __forceinline__ float row_exponent(float x0, float x1, float &back) {
+    float most = fmaxf(fabsf(x0), fabsf(x1));
+    for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
+    back = __uint_as_float((uint32_t)(127 + e) << 23);
+    return __uint_as_float((uint32_t)(127 - e) << 23);
+}
+// a product that is rounded by itself, not inside of the sum that follows: with logits past 2^24 the exact product can be far
+// enough above the rounded maximum for exp2 to overflow
+__device__ __forceinline__ float rounded_product(float x, float y) {
+#pragma clang fp contract(off)
+    return x * y;
+}
+// whether a partial counts, and 1 / its sum.  A paged row with a sum that is no number becomes NaN, elsewhere such partials are left out.
+template <bool PAGED> __device__ __forceinline__ bool part_counts(float l) { return PAGED ? !(l <= 0.0f) : l > 0.0f; }
+template <bool PAGED> __device__ __forceinline__ float part_inverse(float l) { return PAGED ? (l == 0.0f ? 0.0f : 1.0f / l) : l > 0.0f ? 1.0f / l : 0.0f; }
+// a query row's two values of this lane
+__device__ __forceinline__ void paged_query(const AttnArgs &a, const PagedPass &g, int row, int lane, float &x0, float &x1) {
+    row = max(min(row, g.rows - 1), 0);
+    const int t = (int)a.pg.heads_div.div((uint32_t)row), h = row - t * (int)a.pg.heads_div.d;
+    const int64_t at = (g.n ? g.row0 + t : 0) * a.pg.q_token + (int64_t)(g.kvh * (int)a.pg.heads_div.d + h) * a.pg.q_head + 2 * lane;
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint16_t *>(a.q) + at);
+    x0 = a.pg.bf16 ? __uint_as_float(w << 16) : __half2float(__ushort_as_half((unsigned short)(w & 0xffff)));
+    x1 = a.pg.bf16 ? __uint_as_float(w & 0xFFFF0000u) : __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+}
 
 constexpr int KFMT_TURBO = 0, KFMT_Q8 = 1;
 constexpr unsigned long long SKIP_COUNT_MASK = (1ull << 40) - 1ull;  // count bits of a Sparse-V slot; the rest is a nonce tag
@@ -233,7 +324,7 @@ __device__ __forceinline__ void wait_stores() { asm volatile("s_waitcnt vmcnt(0)
 struct MergedPart {
     float M, L, o0, o1;
 };
-template <int NP, int NHD>
+template <int NP, int NHD, bool PAGED>
 __device__ __forceinline__ void merge_few(const float *ml0, const float *po0, int ML, int PO, const int (&head)[NHD], int p_lo, int n, int lane,
                                           MergedPart (&r)[NHD]) {
     float2 ml[NHD][NP], v[NHD][NP];
@@ -251,16 +342,17 @@ __device__ __forceinline__ void merge_few(const float *ml0, const float *po0, in
         r[k] = MergedPart{-INFINITY, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int p = 0; p < NP; ++p)
-            if (ml[k][p].y > 0.0f) r[k].M = fmaxf(r[k].M, ml[k][p].x);
+            if (part_counts<PAGED>(ml[k][p].y)) r[k].M = fmaxf(r[k].M, ml[k][p].x);
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            const float w = ml[k][p].y > 0.0f ? __builtin_amdgcn_exp2f(ml[k][p].x - r[k].M) : 0.0f;
+            const float w = part_counts<PAGED>(ml[k][p].y) ? __builtin_amdgcn_exp2f(ml[k][p].x - r[k].M) : 0.0f;
             r[k].L = fmaf(ml[k][p].y, w, r[k].L);
             r[k].o0 = fmaf(v[k][p].x, w, r[k].o0);
             r[k].o1 = fmaf(v[k][p].y, w, r[k].o1);
         }
     }
 }
+template <bool PAGED>
 __device__ __forceinline__ MergedPart merge_range(const float *ml0, const float *po0, int ML, int PO, int head, int p_lo, int p_hi,
                                                   int lane) {
     MergedPart r{-INFINITY, 0.0f, 0.0f, 0.0f};
@@ -269,9 +361,9 @@ __device__ __forceinline__ MergedPart merge_range(const float *ml0, const float 
     if (n <= 16) {
         const int hd[1] = {head};
         MergedPart one[1];
-        if (n <= 4) merge_few<4, 1>(ml0, po0, ML, PO, hd, p_lo, n, lane, one);
-        else if (n <= 8) merge_few<8, 1>(ml0, po0, ML, PO, hd, p_lo, n, lane, one);
-        else merge_few<16, 1>(ml0, po0, ML, PO, hd, p_lo, n, lane, one);
+        if (n <= 4) merge_few<4, 1, PAGED>(ml0, po0, ML, PO, hd, p_lo, n, lane, one);
+        else if (n <= 8) merge_few<8, 1, PAGED>(ml0, po0, ML, PO, hd, p_lo, n, lane, one);
+        else merge_few<16, 1, PAGED>(ml0, po0, ML, PO, hd, p_lo, n, lane, one);
         return one[0];
     }
     {
@@ -280,7 +372,7 @@ __device__ __forceinline__ MergedPart merge_range(const float *ml0, const float 
             float m = -INFINITY;
             if (p < p_hi) {
                 const float2 e = ld_dev2(ml0 + p * ML + head * 2);
-                if (e.y > 0.0f) m = e.x;
+                if (part_counts<PAGED>(e.y)) m = e.x;
             }
             for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
             r.M = fmaxf(r.M, m);
@@ -291,7 +383,7 @@ __device__ __forceinline__ MergedPart merge_range(const float *ml0, const float 
             if (p < p_hi) {
                 const float2 e = ld_dev2(ml0 + p * ML + head * 2);
                 l = e.y;
-                w = l > 0.0f ? __builtin_amdgcn_exp2f(e.x - r.M) : 0.0f;
+                w = part_counts<PAGED>(l) ? __builtin_amdgcn_exp2f(e.x - r.M) : 0.0f;
             }
             float lw = l * w;
             for (int o = 32; o > 0; o >>= 1) lw += __shfl_xor(lw, o);
@@ -321,7 +413,26 @@ __device__ __forceinline__ MergedPart merge_range(const float *ml0, const float 
 
 // A head's normalised output in the V rotation's domain (two dims per lane) -> its output row.  s1, s2: this lane's signs of the V
 // rotation (unused where V rows are stored unrotated).
-__device__ __forceinline__ void write_row(const AttnArgs &a, int group, int head_off, int head, float o0, float o1, float2 s1, float2 s2, int lane) {
+template <bool PAGED> __device__ __forceinline__ void write_row(const AttnArgs &a, int group, int head_off, int head, float o0, float o1, float2 s1, float2 s2, int lane) {
+    if constexpr (PAGED) {
+        const PagedPass g = paged_pass(a, group, head_off, 1);
+        if (head_off + head >= g.rows) return;
+        o0 *= a.pg.v_unscale;
+        o1 *= a.pg.v_unscale;
+        if (a.vs1) {
+            o0 *= s2.x;
+            o1 *= s2.y;
+            wht128_wave(o0, o1, lane);
+            o0 *= s1.x * RSQRT128;
+            o1 *= s1.y * RSQRT128;
+        }
+        const int t = (int)a.pg.heads_div.div((uint32_t)(head_off + head)), h = head_off + head - t * (int)a.pg.heads_div.d, per = (int)a.pg.heads_div.d;
+        const int64_t row = (g.row0 + t) * ((int64_t)per * a.pg.r.p.n_kv_heads) + g.kvh * per + h;
+        const uint32_t lo = a.pg.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o0) : __builtin_bit_cast(uint16_t, (_Float16)o0);
+        const uint32_t hi = a.pg.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o1) : __builtin_bit_cast(uint16_t, (_Float16)o1);
+        reinterpret_cast<uint32_t *>(a.out)[row * 64 + lane] = lo | (hi << 16);
+        return;
+    }
     // heads of 256 dims: partial row 4 dh + i is dims 128 dh .. 128 dh + 127 of head i
     const int hq = a.d256 ? (head & 3) : head;
     if (head_off + hq >= a.q_group) return;   // a repeated head of a group with fewer left
@@ -341,16 +452,17 @@ __device__ __forceinline__ void write_row(const AttnArgs &a, int group, int head
 // partials, and joins their results through `lds` (free LDS of 132 floats per wavefront; unused otherwise); one with fewer
 // wavefronts than heads has the loads of two heads in flight together: the merge runs at the very end of the launch, so its
 // trips to memory are the launch's tail.
-template <int HG>
+template <int HG, bool PAGED>
 __device__ __forceinline__ void merge_group(const AttnArgs &a, int group, int pgroup, int head_off, int n_parts, int tid, int n_waves,
                                             float *lds, float2 s1, float2 s2) {
     constexpr int NH = 4 * HG, ML = 2 * NH, PO = 128 * NH;  // heads, (m, l) floats and output floats of one partial
     const int lane = tid & 63, wave = tid >> 6;
-    const float *ml0 = a.part_ml + (int64_t)pgroup * n_parts * ML;
-    const float *po0 = a.part_o + (int64_t)pgroup * n_parts * PO;
+    const int64_t at = (int64_t)pgroup * (PAGED ? a.wgs_per_group : n_parts);
+    const float *ml0 = a.part_ml + at * ML;
+    const float *po0 = a.part_o + at * PO;
     auto finish = [&](int head, MergedPart r) {
-        const float invL = r.L > 0.0f ? 1.0f / r.L : 0.0f;
-        write_row(a, group, head_off, head, r.o0 * invL, r.o1 * invL, s1, s2, lane);
+        const float invL = part_inverse<PAGED>(r.L);
+        write_row<PAGED>(a, group, head_off, head, r.o0 * invL, r.o1 * invL, s1, s2, lane);
     };
     auto head_exists = [&](int head) { return head_off + (a.d256 ? (head & 3) : head) < a.q_group; };
     const int n_sub = n_waves >= 2 * NH && n_parts > 4 ? n_waves / NH : 1;
@@ -359,21 +471,21 @@ __device__ __forceinline__ void merge_group(const AttnArgs &a, int group, int pg
             for (int head = wave; head < NH; head += 2 * n_waves) {
                 const int hd[2] = {head, min(head + n_waves, NH - 1)};
                 MergedPart two[2];
-                merge_few<8, 2>(ml0, po0, ML, PO, hd, 0, n_parts, lane, two);
+                merge_few<8, 2, PAGED>(ml0, po0, ML, PO, hd, 0, n_parts, lane, two);
                 finish(head, two[0]);
                 if (head + n_waves < NH) finish(head + n_waves, two[1]);
             }
             return;
         }
         for (int head = wave; head < NH; head += n_waves)
-            if (head_exists(head)) finish(head, merge_range(ml0, po0, ML, PO, head, 0, n_parts, lane));
+            if (head_exists(head)) finish(head, merge_range<PAGED>(ml0, po0, ML, PO, head, 0, n_parts, lane));
         return;
     }
     const int head = wave % NH, sub = wave / NH;
     const int per = (n_parts + n_sub - 1) / n_sub;
     const bool mine = sub < n_sub && head_exists(head);
     MergedPart r{-INFINITY, 0.0f, 0.0f, 0.0f};
-    if (mine) r = merge_range(ml0, po0, ML, PO, head, min(sub * per, n_parts), min(sub * per + per, n_parts), lane);
+    if (mine) r = merge_range<PAGED>(ml0, po0, ML, PO, head, min(sub * per, n_parts), min(sub * per + per, n_parts), lane);
     float *slot = lds + (head * n_sub + (sub < n_sub ? sub : 0)) * 132;
     if (mine) {
         *reinterpret_cast<float2 *>(slot + 2 * lane) = make_float2(r.o0, r.o1);
@@ -387,11 +499,11 @@ __device__ __forceinline__ void merge_group(const AttnArgs &a, int group, int pg
         const float *s0 = lds + head * n_sub * 132;
         float M = -INFINITY;
         for (int k = 0; k < n_sub; ++k)
-            if (s0[k * 132 + 129] > 0.0f) M = fmaxf(M, s0[k * 132 + 128]);
+            if (part_counts<PAGED>(s0[k * 132 + 129])) M = fmaxf(M, s0[k * 132 + 128]);
         MergedPart t{M, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < n_sub; ++k) {
             const float l = s0[k * 132 + 129];
-            const float w = l > 0.0f ? __builtin_amdgcn_exp2f(s0[k * 132 + 128] - M) : 0.0f;
+            const float w = part_counts<PAGED>(l) ? __builtin_amdgcn_exp2f(s0[k * 132 + 128] - M) : 0.0f;
             const float2 o = *reinterpret_cast<const float2 *>(s0 + k * 132 + 2 * lane);
             t.L = fmaf(l, w, t.L);
             t.o0 = fmaf(o.x, w, t.o0);
@@ -405,7 +517,7 @@ __device__ __forceinline__ void merge_group(const AttnArgs &a, int group, int pg
 // slot).  A wavefront's slot: per set of four heads out[4][128] relative to its own maximum, then (m, l)[4].  Every thread takes
 // 1 to 4 neighbouring values and has the reads of all W slots in flight before it uses the first: a loop of LDS round trips per
 // value made this 2.2 us of a step of four wavefronts and 3.4 us with eight heads.
-template <int HG, int W, class Slot>
+template <int HG, int W, bool PAGED, class Slot>
 __device__ __forceinline__ void combine_waves_of(Slot slot, int wave0, int tid_g, float *po, float *pml, bool only) {
     constexpr int E = 512 * HG, PER = E / (64 * W), VW = PER >= 4 ? 4 : PER >= 2 ? 2 : 1;
     typedef float vec_t __attribute__((ext_vector_type(VW)));
@@ -422,18 +534,18 @@ __device__ __forceinline__ void combine_waves_of(Slot slot, int wave0, int tid_g
         float M = -INFINITY, L = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; ++w)
-            if (ml[w].y > 0.0f) M = fmaxf(M, ml[w].x);   // wavefronts that saw an unmasked position
+            if (part_counts<PAGED>(ml[w].y)) M = fmaxf(M, ml[w].x);   // wavefronts that saw an unmasked position
         vec_t sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const bool seen = ml[w].y > 0.0f;   // false for a sum that is not a number, too: it stays out of the others'
+            const bool seen = part_counts<PAGED>(ml[w].y);
             const float f = seen ? __builtin_amdgcn_exp2f(ml[w].x - M) : 0.0f;
             L = seen ? fmaf(ml[w].y, f, L) : L;
 #pragma unroll
             for (int i = 0; i < VW; ++i) sum[i] = fmaf(v[w][i], f, sum[i]);
         }
         if (only) {
-            *reinterpret_cast<vec_t *>(slot(wave0) + src) = sum * (L > 0.0f ? 1.0f / L : 0.0f);   // no other thread reads this place
+            *reinterpret_cast<vec_t *>(slot(wave0) + src) = sum * part_inverse<PAGED>(L);   // no other thread reads this place
         } else {
             if constexpr (VW == 1) st_dev(po + e, sum[0]);
             else
@@ -443,20 +555,20 @@ __device__ __forceinline__ void combine_waves_of(Slot slot, int wave0, int tid_g
         }
     }
 }
-template <int HG, class Slot>
+template <int HG, bool PAGED, class Slot>
 __device__ __forceinline__ void combine_waves(Slot slot, int gw, int wave0, int tid_g, float *po, float *pml, bool only) {
     switch (gw) {   // the counts that attn_plan makes: powers of two, with eight heads also twelve and its halves
-        case 1: combine_waves_of<HG, 1>(slot, wave0, tid_g, po, pml, only); break;
-        case 2: combine_waves_of<HG, 2>(slot, wave0, tid_g, po, pml, only); break;
-        case 4: combine_waves_of<HG, 4>(slot, wave0, tid_g, po, pml, only); break;
-        case 8: combine_waves_of<HG, 8>(slot, wave0, tid_g, po, pml, only); break;
+        case 1: combine_waves_of<HG, 1, PAGED>(slot, wave0, tid_g, po, pml, only); break;
+        case 2: combine_waves_of<HG, 2, PAGED>(slot, wave0, tid_g, po, pml, only); break;
+        case 4: combine_waves_of<HG, 4, PAGED>(slot, wave0, tid_g, po, pml, only); break;
+        case 8: combine_waves_of<HG, 8, PAGED>(slot, wave0, tid_g, po, pml, only); break;
         default:
             if constexpr (HG == 1) {
-                combine_waves_of<HG, 16>(slot, wave0, tid_g, po, pml, only);
+                combine_waves_of<HG, 16, PAGED>(slot, wave0, tid_g, po, pml, only);
             } else {
-                if (gw == 3) combine_waves_of<HG, 3>(slot, wave0, tid_g, po, pml, only);
-                else if (gw == 6) combine_waves_of<HG, 6>(slot, wave0, tid_g, po, pml, only);
-                else combine_waves_of<HG, 12>(slot, wave0, tid_g, po, pml, only);
+                if (gw == 3) combine_waves_of<HG, 3, PAGED>(slot, wave0, tid_g, po, pml, only);
+                else if (gw == 6) combine_waves_of<HG, 6, PAGED>(slot, wave0, tid_g, po, pml, only);
+                else combine_waves_of<HG, 12, PAGED>(slot, wave0, tid_g, po, pml, only);
             }
     }
 }
@@ -486,11 +598,11 @@ __device__ __forceinline__ void install_tag(const AttnArgs &a, unsigned long lon
 // arrive merges the partials and writes the output rows.  gw wavefronts from wave0 on work on the group (tid_g numbers their
 // threads); lds: 132 floats of LDS per wavefront for merge_group, free once the slots have been read; skipped: Sparse V, the
 // workgroup's count in LDS.
-template <int HG, bool SPARSE, class Slot>
+template <int HG, bool SPARSE, bool PAGED = false, class Slot>
 __device__ __forceinline__ void finish_group(const AttnArgs &a, Slot slot, int group, int pgroup, int head_off, int n_parts, int part, int tid,
                                              int tid_g, int gw, int wave0, float *lds, const uint32_t *skipped) {
     constexpr int NH = 4 * HG;
-    const int lane = tid & 63;
+    const int lane = tid & 63, stride = PAGED ? a.wgs_per_group : n_parts;   // a paged group can have fewer partials than places for them
     // the V rotation's signs, requested before the waits below
     float2 s1 = make_float2(1.0f, 1.0f), s2 = s1;
     if (a.vs1) {
@@ -498,8 +610,8 @@ __device__ __forceinline__ void finish_group(const AttnArgs &a, Slot slot, int g
         s2 = *reinterpret_cast<const float2 *>(a.vs2 + 2 * lane);
     }
     __syncthreads();   // every slot (and the skipped count) is written
-    const int64_t at = (int64_t)pgroup * n_parts + part;
-    combine_waves<HG>(slot, gw, wave0, tid_g, a.part_o + at * NH * 128, a.part_ml + at * NH * 2, n_parts == 1);
+    const int64_t at = (int64_t)pgroup * stride + part;
+    combine_waves<HG, PAGED>(slot, gw, wave0, tid_g, a.part_o + at * NH * 128, a.part_ml + at * NH * 2, n_parts == 1);
     if constexpr (SPARSE) {
         // one slot per workgroup, added up by the merging workgroups: thousands of wavefronts finishing together
         // on one atomic would queue for longer than the kernel's own tail, and nothing needs clearing
@@ -512,7 +624,7 @@ __device__ __forceinline__ void finish_group(const AttnArgs &a, Slot slot, int g
         // merges, and every other partial was complete in memory before its owner's increment, hence before this one's.
         __shared__ int i_am_last;
         if (tid == 0) {
-            const unsigned long long before = __hip_atomic_fetch_add(arrival_counter(a, pgroup, n_parts), 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const unsigned long long before = __hip_atomic_fetch_add(arrival_counter(a, pgroup, PAGED ? PAGED_COUNTER_STEP : stride), 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             i_am_last = (int)(before & ARRIVAL_COUNT_MASK) + 1 == n_parts;
         }
         __syncthreads();
@@ -536,15 +648,15 @@ __device__ __forceinline__ void finish_group(const AttnArgs &a, Slot slot, int g
         }
     }
     if (n_parts > 1) {
-        merge_group<HG>(a, group, pgroup, head_off, n_parts, tid, gw, lds, s1, s2);   // one group per workgroup then
+        merge_group<HG, PAGED>(a, group, pgroup, head_off, n_parts, tid, gw, lds, s1, s2);   // one group per workgroup then
     } else {
         const float *rows = slot(wave0);
         for (int head = tid_g >> 6; head < NH; head += gw) {
             const float2 o = *reinterpret_cast<const float2 *>(rows + (head >> 2) * MERGE_FLOATS + (head & 3) * 128 + 2 * lane);
-            write_row(a, group, head_off, head, o.x, o.y, s1, s2, lane);
+            write_row<PAGED>(a, group, head_off, head, o.x, o.y, s1, s2, lane);
         }
     }
-    if (n_parts > 1 && tid == 0) st_dev(arrival_counter(a, pgroup, n_parts), 0ull);  // a replay of a captured launch (same tag) starts from zero
+    if (n_parts > 1 && tid == 0) st_dev(arrival_counter(a, pgroup, PAGED ? PAGED_COUNTER_STEP : stride), 0ull);  // a replay of a captured launch (same tag) starts from zero
     if constexpr (SPARSE) {
         if (a.poll_slots) {
             if (!__syncthreads_and(all_in)) return;
@@ -572,5 +684,9 @@ bool tqk_launch_decode_turbo(const tqattn::AttnArgs &a, int kb, int vb, bool sha
                              hipStream_t s);
 int tqk_decode_turbo_lds(int kb, int vb, bool share);
 bool tqk_launch_decode_q8(const tqattn::AttnArgs &a, int kb, int vb, int hg, bool sparse, dim3 grid, unsigned wg, size_t lds, hipStream_t s);
+unsigned long long tqk_attn_nonce();   // AttnArgs::nonce of a launch
+// attn_paged_kernels.hip and attn_turbo_kernels.hip: the same over a paged cache, without a bias or Sparse V
+bool tqk_launch_paged(const tqattn::AttnArgs &a, int kb, int vb, bool share, int hg, dim3 grid, unsigned wg, size_t lds, hipStream_t s);
+bool tqk_launch_paged_turbo(const tqattn::AttnArgs &a, int kb, int vb, bool share, int n_heads, dim3 grid, int waves, hipStream_t s);
 bool tqk_launch_decode_256(const tqattn::AttnArgs &a, int kb, int vb, bool share, bool sparse, dim3 grid, unsigned wg, size_t lds,
                            hipStream_t s);

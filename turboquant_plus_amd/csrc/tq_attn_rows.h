@@ -193,6 +193,8 @@ __host__ __device__ constexpr int max_waves_per_workgroup(int vbits, int hg, boo
 // just requested, at the top of every tile (4 x 20 000 tokens, turbo3, Sparse V: kernel 24.6 -> 22.6 us; 4 x 16 groups at 6000 tokens 15.1 ->
 // 14.6; one user at 4000 10.8 -> 10.5).
 constexpr int BIAS_NONE = 0, BIAS_LIST = 1, BIAS_DENSE = 2, BIAS_BOTH = BIAS_LIST | BIAS_DENSE;
+// no bias, over a paged cache: a group's rows, context and blocks come from the tables (AttnArgs::pg), each row has a limit of its own
+constexpr int BIAS_PAGED = 4;
 // D256: heads of 256 dims.  A token is rows 2 token and 2 token + 1 of caches that are
 // otherwise those of 128-dim heads with twice the tokens; a 64-row tile is 32 tokens.  The two sets of HG = 2 are
 // then the output's two halves of one set of four heads: one softmax, two accumulator sets.
@@ -202,6 +204,8 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
     // (256-dim heads on turbo K rows: four wavefronts per SIMD = two workgroups of eight per CU, i.e. at most 128 registers - the
     // variant sits at 119-136 without the bound, and one register over 128 halves its occupancy)
     static_assert(!D256 || HG == 2, "256-dim heads: two accumulator sets, the output's halves");
+    constexpr bool PAGED = BIAS == BIAS_PAGED;
+    static_assert(!PAGED || (!SPARSE && !D256), "what a paged step has");
     constexpr bool LIST = (BIAS & BIAS_LIST) != 0, DENSE = (BIAS & BIAS_DENSE) != 0;
     constexpr int HQ = D256 ? 1 : HG;   // sets of four heads whose logits and softmax state the wavefront keeps
     constexpr int KROW_DW = KFMT == KFMT_TURBO ? 4 * KBITS : 32;
@@ -214,6 +218,7 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
     // group's rotated queries (a region of its own: the tables are built while the queries are still on their way)
     constexpr int LUT_TOTAL = KLUT_BYTES + (SHARE ? 0 : lut_bytes(VBITS));
     __shared__ __attribute__((aligned(16))) char smem[LUT_TOTAL > 16 ? LUT_TOTAL : 16];
+    __shared__ float row_scale[PAGED ? 64 : 1];   // PAGED: [group of the workgroup][head], a query row's power of two and the logit scale
     __shared__ uint32_t lead;  // tiles finished by the wavefront that is furthest ahead
     __shared__ uint32_t skipped;  // Sparse V: (query, position) pairs skipped by this workgroup
     char *klut_s = smem;
@@ -230,9 +235,10 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
     const int wave_g = a.gpw > 1 ? (wave & (gw - 1)) : wave, wave0 = wave - wave_g;
     const int gidx = a.gpw > 1 ? (wave >> a.gw_shift) : 0;   // this wavefront's group among the workgroup's
     const int tid_g = tid - 64 * wave0;
-    const int wgs_per_group = a.wgs_per_group;
-    const int group = __builtin_amdgcn_readfirstlane(a.gpw > 1 ? (int)blockIdx.x * a.gpw + gidx : (int)(blockIdx.x / wgs_per_group));
-    const int part = a.gpw > 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(blockIdx.x % wgs_per_group));
+    const int places = a.wgs_per_group;   // partials that a group has room for
+    int wgs_per_group = places;
+    const int group = __builtin_amdgcn_readfirstlane(a.gpw > 1 ? (int)blockIdx.x * a.gpw + gidx : (int)(blockIdx.x / places));
+    const int part = a.gpw > 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(blockIdx.x % places));
     const int pass_y = HG == 2 ? (int)blockIdx.y : 0;   // one set of four heads is always one pass
     const int head_off = a.head_off + pass_y * a.pass_heads, pgroup = pass_y * a.n_groups + group;
     const int split = part * n_waves + wave_g;  // index of this wavefront's partial
@@ -250,9 +256,17 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
         n_tiles = ((D256 ? 2 : 1) * tokens_now + 63) >> 6;
         tiles_per_split = (n_tiles + a.n_splits - 1) / a.n_splits;
     }
+    PagedPass pg{};
+    int paged_begin = 0, paged_end = 0;
+    if constexpr (PAGED) {
+        pg = paged_pass(a, group, head_off, 4 * HG);
+        tokens_now = pg.most;
+        n_tiles = (tokens_now + 63) >> 6;
+        if (!paged_tiles(a, pg, n_tiles, part, wave_g, wgs_per_group, paged_begin, paged_end)) return;
+    }
     const int rows_now = (D256 ? 2 : 1) * tokens_now;   // rows of the caches that hold the context
-    const int t_begin = split * tiles_per_split;
-    const int t_end = min(t_begin + tiles_per_split, n_tiles);
+    const int t_begin = PAGED ? paged_begin : split * tiles_per_split;
+    const int t_end = PAGED ? paged_end : min(t_begin + tiles_per_split, n_tiles);
     const int b4 = lane & ~3;  // 4 * block index
     const int j = lane & 3;    // query head of the logits this lane holds; sub-row for V
     // K row of the tile that this lane owns, and the tile row of element i of its logits (e4 + es * i)
@@ -264,6 +278,16 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
 
     const uint8_t *kbase = a.k + (int64_t)group * a.blocks_per_seq * KBLOCK;
     const uint8_t *vbase = a.v + (int64_t)group * a.blocks_per_seq * VBLOCK;
+    // the block of a tile: of the sequence's own, or (PAGED) of its page, whose number is looked up two tiles ahead
+    auto page_of = [&](int tile) { return PAGED ? scalar_entry(pg.table, __builtin_amdgcn_readfirstlane(tile >> 1)) : 0; };
+    auto is_page = [&](int page) { return page >= 0 && page < a.pg.r.p.n_pages; };
+    auto block_no = [&](int tile, int page) -> int64_t {
+        return PAGED ? (int64_t)(is_page(page) ? page : 0) * a.pg.r.p.n_kv_heads + pg.kvh : (int64_t)(tile >> 1);
+    };
+    if constexpr (PAGED) {
+        kbase = a.k;
+        vbase = a.v;
+    }
     const char *klut_b = klut_s + (TQ_PAIRTAB3 && KFMT == KFMT_TURBO && KBITS == 3 ? 4 * lane : 0);
     const char *vlut_b = vlut_s + (TQ_PAIRTAB3 && VBITS == 3 ? 4 * lane : 0);
 
@@ -278,8 +302,8 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
     uint32_t kw[KROW_DW];
     uint32_t vw[4 * VBITS];
     // K: this lane's token's fp16 norm (turbo) or its four fp16 block scales (q8_0-style)
-    auto load_knorm = [&](int tile) -> uint2 {
-        const uint8_t *kb = kbase + (int64_t)(tile >> 1) * KBLOCK;
+    auto load_knorm = [&](int tile, int page) -> uint2 {
+        const uint8_t *kb = kbase + block_no(tile, page) * KBLOCK;
         const int r = (tile & 1) * 64 + krow;
         if constexpr (KFMT == KFMT_TURBO)
             return make_uint2(reinterpret_cast<const uint16_t *>(kb + TQ_ROWS_PER_BLOCK * 16 * KBITS)[r], 0u);
@@ -287,9 +311,9 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
             return *reinterpret_cast<const uint2 *>(kb + 8 * 2048 + 8 * r);
     };
     // V: fp16 norms of this lane's four tokens 4b..4b+3, or their q8_0-style scales ([tile][32-dim block][token])
-    auto load_vnorm = [&](int tile) -> VSide<VBITS> {
+    auto load_vnorm = [&](int tile, int page) -> VSide<VBITS> {
         VSide<VBITS> r;
-        const uint8_t *side = vbase + (int64_t)(tile >> 1) * VBLOCK + TQ_ROWS_PER_BLOCK * 16 * VBITS;
+        const uint8_t *side = vbase + block_no(tile, page) * VBLOCK + TQ_ROWS_PER_BLOCK * 16 * VBITS;
         if constexpr (VBITS == 8 && D256) {
             const int bh = lane >> 5;
 #pragma unroll
@@ -315,20 +339,23 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
         return r;
     };
     unsigned long long arrivals_seen = 0ull;
-    if (wgs_per_group > 1 && tid == 0) arrivals_seen = ld_dev(arrival_counter(a, pgroup, wgs_per_group));
+    if (wgs_per_group > 1 && tid == 0) arrivals_seen = ld_dev(arrival_counter(a, pgroup, PAGED ? PAGED_COUNTER_STEP : places));
     uint2 kn = make_uint2(0u, 0u);
     VSide<VBITS> gvu;
 #pragma unroll
     for (auto &e : gvu.v) e = make_uint2(0u, 0u);
     int tile = t_begin;
+    int page = 0, page_n = 0;    // PAGED: of this tile and the next
     if (tile < t_end) {
+        page = page_of(tile);
+        page_n = page_of(min(tile + 1, t_end - 1));
         const int row0 = (tile & 1) * 64 + lane;
-        const uint8_t *kb = kbase + (int64_t)(tile >> 1) * KBLOCK;
+        const uint8_t *kb = kbase + block_no(tile, page) * KBLOCK;
         if constexpr (KFMT == KFMT_TURBO) load_row<KBITS>(kb, (tile & 1) * 64 + krow, kw);
         else load_row<8>(kb, (tile & 1) * 64 + krow, kw);
-        kn = load_knorm(tile);
-        load_row<VBITS>(vbase + (int64_t)(tile >> 1) * VBLOCK, row0, vw);
-        gvu = load_vnorm(tile);
+        kn = load_knorm(tile, page);
+        load_row<VBITS>(vbase + block_no(tile, page) * VBLOCK, row0, vw);
+        gvu = load_vnorm(tile, page);
     }
     if (tid == 0) {
         lead = 0;
@@ -344,6 +371,10 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
     // The group's four queries are rotated by the first wavefronts (one 128-point butterfly per
     // head, two values per lane), scaled and parked as fp16 in 1 KB of LDS for everybody.
     auto load_q = [&](int h, float &x0, float &x1) {
+        if constexpr (PAGED) {
+            paged_query(a, pg, head_off + h, lane, x0, x1);
+            return;
+        }
         // heads past the group's last one repeat it (their results are not written)
         const int64_t e = D256 ? ((int64_t)group * a.q_group + min(head_off + (h & 3), a.q_group - 1)) * 256 + 128 * (h >> 2) + 2 * lane
                                : ((int64_t)group * a.q_group + min(head_off + h, a.q_group - 1)) * 128 + 2 * lane;
@@ -417,6 +448,13 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
         _Float16 *qw = reinterpret_cast<_Float16 *>(q_stage) + h * 128;
         float x0 = xq0, x1 = xq1;
         if (h != wave_g) load_q(h, x0, x1);
+        if constexpr (PAGED) {
+            float back;
+            const float f = row_exponent(x0, x1, back);
+            x0 *= f;
+            x1 *= f;
+            if (lane == 0) row_scale[gidx * 4 * HG + h] = KFMT == KFMT_Q8 ? back : back * a.scale_log2e;
+        }
         if (a.ks1) {
             x0 *= a.ks1[2 * lane];
             x1 *= a.ks1[2 * lane + 1];
@@ -432,11 +470,11 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
         // fp16 query goes in as it is, so that its products with the int8 values are exact, and the logit scale
         // joins the rows' block scales in fp32 (rounding the scaled query would move logits of rows with large
         // channels by several 1e-3, which a peaked softmax over a long context turns into output error)
-        const float qscale = KFMT == KFMT_Q8 ? 1.0f : a.scale_log2e;
+        const float qscale = KFMT == KFMT_Q8 || PAGED ? 1.0f : a.scale_log2e;
         qw[p0] = (_Float16)(x0 * qscale);
         qw[p1] = (_Float16)(x1 * qscale);
     }
-    if (wgs_per_group > 1 && tid == 0) install_tag(a, arrival_counter(a, pgroup, wgs_per_group), arrivals_seen);
+    if (wgs_per_group > 1 && tid == 0) install_tag(a, arrival_counter(a, pgroup, PAGED ? PAGED_COUNTER_STEP : places), arrivals_seen);
     __syncthreads();
     half4_t qa[HG][2];
     half4_t qa4[4];   // 256-dim heads: dim groups b, b + 8, b + 16, b + 24 of this half-wavefront's half of the query
@@ -486,15 +524,22 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
     unsigned nskip = 0;  // Sparse V: skipped (query, position) pairs of this wavefront (wave-uniform: counted from lane masks)
     bool v_ahead = true;  // Sparse V: this tile's V row was requested while the previous tile was processed
 
+    int lim[HG];   // PAGED: the positions that this lane's heads see
+#pragma unroll
+    for (int hg = 0; hg < HG; ++hg) lim[hg] = PAGED && pg.rows > 0 ? paged_limit(a, pg, min(head_off + 4 * hg + j, pg.rows - 1)) : 0;
+    float f_row[HG];
+#pragma unroll
+    for (int hg = 0; hg < HG; ++hg) f_row[hg] = PAGED ? row_scale[gidx * 4 * HG + 4 * hg + j] : 1.0f;
     unsigned long long head_ok[HG];  // lanes whose head (lane % 4 of each set) exists in this pass
 #pragma unroll
     for (int hg = 0; hg < HG; ++hg) head_ok[hg] = __builtin_amdgcn_ballot_w64(head_off + 4 * hg + j < a.q_group);
 #pragma unroll 1
     while (tile < t_end) {
-        const int64_t blk = tile >> 1;
         const int half = tile & 1;
         const int row = half * 64 + lane;
-        const uint8_t *vb = vbase + blk * VBLOCK;
+        const uint8_t *vb = vbase + block_no(tile, page) * VBLOCK;
+        int page_after = 0;
+        if constexpr (PAGED) page_after = page_of(min(tile + 2, t_end - 1));
 
         {   // issue priority = tiles behind the leader (wave-uniform, so the branches are scalar)
             const uint32_t done = (uint32_t)(tile - t_begin);
@@ -508,8 +553,10 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
         const int tile_n = min(tile_next, t_end - 1);
         const int row_n = tile_next < t_end ? (tile_n & 1) * 64 + lane : 0;  // past the split: every lane the same row
         const int krow_n = tile_next < t_end ? (tile_n & 1) * 64 + krow : 0;
-        const VSide<VBITS> gvu_next = load_vnorm(tile_n);
+        const VSide<VBITS> gvu_next = load_vnorm(tile_n, page_n);
         const int n_valid = rows_now - tile * 64;   // >= 64 except in the sequence's last tile
+        const bool masked = PAGED && (pg.least - tile * 64 < 64 || !is_page(page));   // some head does not see all of the tile
+        const int first_out = PAGED && is_page(page) ? tile * 64 : 0x7FFFFFFF;         // lim - first_out: positions of it that a head sees
         // the bias of this tile was requested a tile ago, like the rows; now the next tile's
         float bias4[HG][4];
 #pragma unroll
@@ -602,10 +649,10 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
                 for (int i = 0; i < 4; ++i) sc[hg][i] = (acc[hg][0][i] * d0 + acc[hg][1][i] * d1) + (acc[hg][2][i] * d2 + acc[hg][3][i] * d3);
         }
         {   // kw is dead now: fetch the next tile's K row into it
-            const uint8_t *kbn = kbase + (int64_t)(tile_n >> 1) * KBLOCK;
+            const uint8_t *kbn = kbase + block_no(tile_n, page_n) * KBLOCK;
             if constexpr (KFMT == KFMT_TURBO) load_row<KBITS>(kbn, krow_n, kw);
             else load_row<8>(kbn, krow_n, kw);
-            kn = load_knorm(tile_n);
+            kn = load_knorm(tile_n, page_n);
         }
         // -> lane (b, j): head j (of each set), tokens 4b..4b+3; then the online softmax in base 2
         float p[HG][4];
@@ -623,8 +670,14 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
             quad_transpose(sc[hg], lane);
             float s[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = BIAS ? sc[hg][i] + bias4[hg][i] : sc[hg][i];
-            if (n_valid < 64) {
+            for (int i = 0; i < 4; ++i) s[i] = PAGED ? rounded_product(sc[hg][i], f_row[hg]) : BIAS ? sc[hg][i] + bias4[hg][i] : sc[hg][i];
+            if constexpr (PAGED) {
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (e4 + i >= lim[hg] - first_out) s[i] = -INFINITY;
+                }
+            } else if (n_valid < 64) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (e4 + es * i >= n_valid) s[i] = -INFINITY;
@@ -705,7 +758,7 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
             // The dims of block b lie in 32-dim block b / 8 (+ 2 for the upper dim half), so the weights carry that
             // block's scale and are broadcast inside each half of the wavefront: token group T is served by block
             // T % 8 of both halves, which therefore also needs the weights of the lane 32 away.
-            auto weights = [&](const float (&w)[4], uint2 sc) {
+            auto weights = [&](const float (&w)[4], uint2 sc, int first, int seen) {   // tokens first .. first + 3, of which those below `seen` count
                 const float s0 = __half2float(__ushort_as_half((unsigned short)(sc.x & 0xffff))) * Q8V_PRESCALE;
                 const float s1 = __half2float(__ushort_as_half((unsigned short)(sc.x >> 16))) * Q8V_PRESCALE;
                 const float s2 = __half2float(__ushort_as_half((unsigned short)(sc.y & 0xffff))) * Q8V_PRESCALE;
@@ -715,6 +768,15 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
                 r[1] = (_Float16)(w[2] * s2);
                 r[2] = (_Float16)(w[1] * s1);
                 r[3] = (_Float16)(w[3] * s3);
+                if constexpr (PAGED) {
+                    if (masked) {   // what a masked place holds may be no number
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = ((i & 1) << 1) | (i >> 1);
+                            r[at] = first + i < seen ? r[at] : (_Float16)0.0f;
+                        }
+                    }
+                }
                 return r;
             };
             const bool upper = lane >= 32;
@@ -726,7 +788,7 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
                 for (int i = 0; i < 4; ++i) ps[i] = __shfl_xor(p[hg][i], 32);
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const half4_t own = weights(p[hg], gvu.v[2 * hf]), swp = weights(ps, gvu.v[2 * hf + 1]);
+                    const half4_t own = weights(p[hg], gvu.v[2 * hf], b4, lim[hg] - first_out), swp = weights(ps, gvu.v[2 * hf + 1], b4 ^ 32, lim[hg] - first_out);
                     a_lo[hg][hf] = upper ? swp : own;
                     a_hi[hg][hf] = upper ? own : swp;
                 }
@@ -760,16 +822,26 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
                 pv[hg][1] = (_Float16)(p[hg][1] * g1);
                 pv[hg][2] = (_Float16)(p[hg][2] * g2);
                 pv[hg][3] = (_Float16)(p[hg][3] * g3);
+                if constexpr (PAGED) {
+                    if (masked) {   // what a masked place holds may be no number
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) pv[hg][i] = e4 + i < lim[hg] - first_out ? pv[hg][i] : (_Float16)0.0f;
+                    }
+                }
             }
             // V row of this lane: dims lane and 64+lane for the tile's 64 tokens; quad 2T + hf =
             // tokens 4T..4T+3 of dim half hf.  Block b = lane/4 of the MFMA covers dims 4b..4b+3 (+64*hf); the
             // weights of token group T sit in block T and are broadcast to every block.
             pv_all<VBITS, HG>(std::make_integer_sequence<int, 16>{}, vw, vlut_b, pv, acc_o);
         }
-        load_row<VBITS>(vbase + (int64_t)(tile_n >> 1) * VBLOCK, row_n, vw);
+        load_row<VBITS>(vbase + block_no(tile_n, page_n) * VBLOCK, row_n, vw);
         v_ahead = true;
         gvu = gvu_next;
         tile = tile_next;
+        if constexpr (PAGED) {
+            page = page_n;
+            page_n = page_after;
+        }
     }
 
     // ---- end of split: the workgroup's wavefronts merge their partials in LDS and write one ------
@@ -799,7 +871,7 @@ __global__ __launch_bounds__(64 * max_waves_per_workgroup(VBITS, HG, KFMT == KFM
         if (lane < 4) *reinterpret_cast<float2 *>(mine + hg * MERGE_FLOATS + 512 + 2 * j) = make_float2(m_run[hg], l_tot[hg]);
     }
     if (SPARSE && lane == 0 && nskip) atomicAdd(&skipped, nskip);
-    finish_group<HG, SPARSE>(a, slot, group, pgroup, head_off, wgs_per_group, part, tid, tid_g, gw, wave0, merge_s, &skipped);
+    finish_group<HG, SPARSE, PAGED>(a, slot, group, pgroup, head_off, wgs_per_group, part, tid, tid_g, gw, wave0, merge_s, &skipped);
 }
 
 // by the bias that the call carries

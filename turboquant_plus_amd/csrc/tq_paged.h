@@ -3,6 +3,13 @@
 #include "tq_internal.h"
 #include "tq_layout.h"
 
+// An entry of a table that no running launch changes, at an index that is the same in all lanes: by a scalar load.  As a vector
+// load it would return behind the rows requested before it, and the wavefront, which needs it at once, would wait for them all.
+__device__ __forceinline__ int32_t scalar_entry(const int32_t *table, int64_t i) {
+    typedef const int32_t __attribute__((address_space(4))) *constant_ptr;
+    return *(constant_ptr)(uintptr_t)(table + i);
+}
+
 struct PagedRows {
     tq_pages p;
     int64_t rows;           // of the new tokens' tensors

@@ -16,6 +16,8 @@
 // across lanes.  `kw` wavefronts of a workgroup share the positions of one row block and join through LDS at the end;
 // n_splits workgroups share them where rows are few, through partial results in memory (32 bits) and k_paged_merge.
 #pragma once
+#include <type_traits>
+
 #include "tq_device.h"
 #include "tq_paged.h"
 
@@ -28,6 +30,10 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 constexpr float RSQRT128 = 0.08838834764831845f;
 
+// How rows are dealt out, by a sequence's most: 32 or 48 to a wavefront that decodes for itself, 128 or 256 to a workgroup
+enum PagedKind { ROWS_32, ROWS_48, CHUNK_128, CHUNK_256 };
+__host__ __device__ constexpr int rows_of(PagedKind k) { return k == ROWS_32 ? 32 : k == ROWS_48 ? 48 : k == CHUNK_128 ? 128 : 256; }
+
 struct PagedAttnArgs {
     PagedRows r;
     const void *q;
@@ -35,12 +41,14 @@ struct PagedAttnArgs {
     int64_t q_token, q_head;
     int bf16, causal, max_context, max_new;
     int group;                   // query heads per KV head
+    int blocks_each;             // 0, or the row blocks that every sequence has
     FastDiv group_div, heads_div;
     const uint8_t *k, *v;
     const uint32_t *klut, *vlut; // pair tables of value_scale times the codebook
     const float *ks1, *ks2, *vs1, *vs2;
     float scale;                 // logits' scale * log2(e) / value_scale of K
     float v_unscale;             // 1 / value_scale of V
+    int share;                   // K's table is V's
     int n_splits, split_tiles;   // of the positions, and 64-position tiles of each
     int kw;                      // wavefronts that share a row block's positions
     float *part_o, *part_ml;     // [row][query head][split]: 128 sums; maximum (log2 units), sum of weights
@@ -63,31 +71,32 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs &a, const Pa
 }
 
 // ---- decode tables ---------------------------------------------------------------------------------
-// 2 and 3 bits: four values per entry (8 bytes), indexed by two neighbouring pair codes; 4 bits: two values per entry
-__host__ __device__ constexpr int table_bytes(int bits) { return bits == 8 ? 0 : bits == 4 ? 1024 : 8 << (4 * bits); }
-template <int BITS> __device__ __forceinline__ void build_table(char *dst, const uint32_t *pairs, int tid, int threads) {
-    if constexpr (BITS == 4) {
-        for (int e = tid; e < 256; e += threads) reinterpret_cast<uint32_t *>(dst)[e] = pairs[e];
-    } else {
-        constexpr int NP = 1 << (2 * BITS);
-        for (int e = tid; e < NP * NP; e += threads) reinterpret_cast<uint2 *>(dst)[e] = make_uint2(pairs[e & (NP - 1)], pairs[e / NP]);
+// Two fp16 values per entry, indexed by a pair code, with C copies next to each other: lanes read their own copy, so that
+// look-ups of a wavefront meet in few banks.
+__host__ __device__ constexpr int pair_table_bytes(int bits, int copies) { return bits == 8 ? 0 : (4 << (2 * bits)) * copies; }
+template <int BITS, int C> __device__ __forceinline__ void build_pair_table(char *dst, const uint32_t *pairs, int tid, int threads) {
+    for (int e = tid; e < (C << (2 * BITS)) / 4; e += threads) {
+        const uint32_t p = pairs[4 * e / C];
+        reinterpret_cast<uint4 *>(dst)[e] = make_uint4(p, p, p, p);
     }
 }
 template <int BITS> __device__ __forceinline__ uint32_t group_tail(const uint32_t (&w)[BITS]) {
     if constexpr (BITS == 3) return (w[0] >> 24) | ((w[1] >> 24) << 8) | ((w[2] >> 24) << 16);
     else return 0u;
 }
-// the four values of quad Q = 0 .. 7 of a pair group
-template <int BITS> __device__ __forceinline__ uint2 group_quad(const uint32_t (&w)[BITS], uint32_t tail, const char *lut, int Q) {
-    if constexpr (BITS == 4) {
-        const uint32_t x = w[Q >> 1];
-        return make_uint2(*reinterpret_cast<const uint32_t *>(lut + field_offset<2>(x, 16 * (Q & 1), 8)),
-                          *reinterpret_cast<const uint32_t *>(lut + field_offset<2>(x, 16 * (Q & 1) + 8, 8)));
-    } else if constexpr (BITS == 2) {
-        return *reinterpret_cast<const uint2 *>(lut + field_offset<3>(w[Q >> 2], 8 * (Q & 3), 8));
-    } else {
-        return *reinterpret_cast<const uint2 *>(lut + (Q < 6 ? field_offset<3>(w[Q >> 1], 12 * (Q & 1), 12) : field_offset<3>(tail, 12 * (Q - 6), 12)));
-    }
+constexpr int log2_of(int x) { return x <= 1 ? 0 : 1 + log2_of(x >> 1); }
+// the two values of pair P = 0 .. 15 of a pair group; copy: 4 (lane % C)
+template <int BITS, int C> __device__ __forceinline__ uint32_t group_pair(const uint32_t (&w)[BITS], uint32_t tail, const char *lut, uint32_t copy, int P) {
+    constexpr int SCALE = 2 + log2_of(C);
+    uint32_t at;
+    if constexpr (BITS == 4) at = field_offset<SCALE>(w[P >> 2], 8 * (P & 3), 8);
+    else if constexpr (BITS == 2) at = field_offset<SCALE>(w[P >> 3], 4 * (P & 7), 4);
+    else at = P < 12 ? field_offset<SCALE>(w[P < 12 ? P >> 2 : 0], 6 * (P & 3), 6) : field_offset<SCALE>(tail, 6 * (P - 12), 6);
+    return *reinterpret_cast<const uint32_t *>(lut + (at | copy));
+}
+// the four values of quad Q = 0 .. 7
+template <int BITS, int C> __device__ __forceinline__ uint2 group_quad(const uint32_t (&w)[BITS], uint32_t tail, const char *lut, uint32_t copy, int Q) {
+    return make_uint2(group_pair<BITS, C>(w, tail, lut, copy, 2 * Q), group_pair<BITS, C>(w, tail, lut, copy, 2 * Q + 1));
 }
 __device__ __forceinline__ half8_t join(uint2 a, uint2 b) { return __builtin_bit_cast(half8_t, make_uint4(a.x, a.y, b.x, b.y)); }
 
@@ -163,69 +172,54 @@ __device__ __forceinline__ void write_out(const PagedAttnArgs &a, float (&o)[32]
     }
 }
 
-__host__ __device__ constexpr int paged_waves(int rb) { return rb == 1 ? 8 : 4; }
-// floats that a wavefront leaves behind for another one to join: 32 RB sums, RB maxima and sums of weights per lane
-__host__ __device__ constexpr int join_floats(int rb) { return 64 * 34 * rb; }
-__host__ __device__ constexpr int paged_lds(int kb, int vb, int rb, bool share) {
-    const int tables = table_bytes(kb) + (share ? 0 : table_bytes(vb)), join = paged_waves(rb) / 2 * join_floats(rb) * 4;
-    return tables > join ? tables : join;
+// Rows r0 .. of a sequence, RB blocks of 16 of them to a wavefront: which they are, their queries, and what the walk leaves.
+struct PagedBlock {
+    PagedSeq seq;
+    PagedSpan span;
+    int n_rows, r0;    // rows of the sequence (tokens times query heads); the block's first
+    bool active;       // it has rows, and positions in this split (the first split also if there are none)
+};
+// Row block `item` (of `rows` rows each) of all sequences
+__device__ __forceinline__ PagedBlock paged_block(const PagedAttnArgs &a, int item, int rows, int split, int &b) {
+    PagedBlock k{{0, 0, 0}, {0, 0}, 0, 0, false};
+    int nth = 0;
+    bool some;
+    b = 0;
+    if (a.blocks_each) {    // one row per sequence: every one has as many row blocks
+        b = item / a.blocks_each;
+        nth = item - b * a.blocks_each;
+        some = b < a.r.p.batch;
+        if (!some) b = 0;
+    } else some = paged_item(a.r, item, [&](int s) { return (min(paged_seq(a.r, s).n, a.max_new) * a.group + rows - 1) / rows; }, b, nth);
+    if (some) {
+        k.seq = paged_seq(a.r, b);
+        k.span = paged_span(a, k.seq);
+        k.n_rows = min(k.seq.n, a.max_new) * a.group;
+        k.r0 = nth * rows;
+        k.active = k.r0 < k.n_rows && (split < k.span.splits || split == 0);
+    }
+    return k;
+}
+// positions that row r sees
+__device__ __forceinline__ int row_limit(const PagedAttnArgs &a, const PagedBlock &k, int r) {
+    const int t = (int)a.group_div.div((uint32_t)r), seen = a.causal ? k.span.ctx - k.seq.n + t + 1 : k.span.ctx;
+    return seen < 0 ? 0 : seen;
 }
 
-// KB, VB: code widths, 8 for q8_0-style rows; RB: blocks of 16 rows per wavefront; SHARE: one table for K and V
-template <int KB, int VB, int RB, bool SHARE>
-__global__ __launch_bounds__(64 * paged_waves(RB)) void k_paged_attn(PagedAttnArgs a) {
-    constexpr int W = paged_waves(RB), TILE = 16 * RB;
-    constexpr int KBLOCK = KB == 8 ? TQ_ROWS_PER_BLOCK * 136 : block_bytes(KB), VBLOCK = VB == 8 ? TQ_ROWS_PER_BLOCK * 136 : block_bytes(VB);
-    __shared__ __attribute__((aligned(16))) char smem[paged_lds(KB, VB, RB, SHARE)];
-    const char *klut = smem, *vlut = SHARE ? smem : smem + table_bytes(KB);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// Queries of RB blocks from row `first` on: 32 values of row n16 of each block, rotated as K's rows are, as fp16 of their size up to
+// a power of two, which joins the logits' scale.  Rows past the last one repeat it.
+template <int KB, int RB>
+__device__ __forceinline__ void load_queries(const PagedAttnArgs &a, const PagedBlock &k, int first, int head, int lane, half8_t (&qf)[RB][4],
+                                             float (&scale)[RB], int (&seen)[RB]) {
     const int n16 = lane & 15, kq = lane >> 4;
-    // neighbouring workgroups have the KV heads of the same rows: with eight of them each die keeps to one head's pages
-    const uint32_t rest = a.heads_div.div(blockIdx.x);
-    const int head = (int)(blockIdx.x - rest * a.heads_div.d);
-    const int split = a.n_splits == 1 ? 0 : (int)(rest % (uint32_t)a.n_splits);
-    const int turn = a.n_splits == 1 ? (int)rest : (int)(rest / (uint32_t)a.n_splits);
-    const int kw = a.kw, part = wave & (kw - 1);
-    const int item = turn * (W / kw) + wave / kw;
-    int b = 0, nth = 0;
-    const bool some = paged_item(a.r, item, [&](int s) { return (min(paged_seq(a.r, s).n, a.max_new) * a.group + TILE - 1) / TILE; }, b, nth);
-    PagedSeq seq{0, 0, 0};
-    PagedSpan span{0, 0};
-    if (some) {
-        seq = paged_seq(a.r, b);
-        span = paged_span(a, seq);
-    }
-    const int n_rows = min(seq.n, a.max_new) * a.group, r0 = nth * TILE;
-    const bool active = some && (split < span.splits || split == 0);
-    // positions that the block's last and first rows see
-    auto limit = [&](int r) {
-        const int t = (int)a.group_div.div((uint32_t)r), seen = a.causal ? span.ctx - seq.n + t + 1 : span.ctx;
-        return seen < 0 ? 0 : seen;
-    };
-    int t_begin = 0, t_end = 0, least = 0;
-    if (active) {
-        least = limit(r0);
-        t_begin = split * a.split_tiles;
-        t_end = min((limit(min(r0 + TILE, n_rows) - 1) + 63) >> 6, t_begin + a.split_tiles);
-        const int each = (max(t_end - t_begin, 0) + kw - 1) / kw;
-        t_begin += part * each;
-        t_end = min(t_end, t_begin + each);
-    }
-    if constexpr (KB != 8) build_table<KB>(smem, a.klut, tid, 64 * W);
-    if constexpr (VB != 8 && !SHARE) build_table<VB>(smem + table_bytes(KB), a.vlut, tid, 64 * W);
-
-    // queries: 32 values of row n16 of each block, rotated as K's rows are, as fp16 of their size up to a power of two
-    half8_t qf[RB][4];
-    float scale[RB];   // of the logits, with that power of two
-    int seen[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        const int r = min(r0 + 16 * rb + n16, max(n_rows - 1, 0));   // rows past the last one repeat it
+        const int r = min(first + 16 * rb + n16, max(k.n_rows - 1, 0));
         const int t = (int)a.group_div.div((uint32_t)r), g = r - t * a.group;
-        seen[rb] = limit(r);
+        seen[rb] = row_limit(a, k, r);
         float x[32];
-        const int64_t at = (seq.row0 + t) * a.q_token + (int64_t)(head * a.group + g) * a.q_head + 32 * kq;
-        if (active) {
+        const int64_t at = (k.seq.row0 + t) * a.q_token + (int64_t)(head * a.group + g) * a.q_head + 32 * kq;
+        if (k.active) {
             const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + at);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -270,51 +264,272 @@ __global__ __launch_bounds__(64 * paged_waves(RB)) void k_paged_attn(PagedAttnAr
                 qf[rb][ks][e] = (_Float16)__builtin_amdgcn_ldexpf(x[8 * ks + from], -ex);
             }
     }
+}
 
-    float4_t o[RB][2][4];
-    float m[RB], l[RB];
+// One tile's logits of a row block, in three steps.  (1) times the tokens' norms, places that do not count out (MASKED: the lane's 16
+// tokens of which the first `sees` do); the row's new maximum.
+template <int KB, bool MASKED, class KNorm>
+__device__ __forceinline__ float logits_max(float4_t (&s)[4], KNorm kn, int sees, float scale, float m) {
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v = s[u][i];
+            if constexpr (KB != 8) v *= kn(4 * u + i);
+            if constexpr (MASKED) v = 4 * u + i < sees ? v : -INFINITY;
+            s[u][i] = v;
+            most = fmaxf(most, v);
+        }
+    return fmaxf(m, over_row_max(most) * scale);
+}
+// (2) the sums of all of a wavefront's row blocks shrink to the new maxima, which they rarely have to
+template <int RB, typename L> __device__ __forceinline__ void move_max(const float (&m_new)[RB], float (&m)[RB], L (&l)[RB], float4_t (&o)[RB][2][4]) {
+    bool moved = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) moved = moved || m_new[rb] != m[rb];
+    if (__builtin_amdgcn_ballot_w64(moved) != 0ull) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const float shrink = m_new[rb] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rb] - m_new[rb]);
+            l[rb] *= shrink;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[rb][e >> 2][e & 3] *= shrink;
+            m[rb] = m_new[rb];
+        }
+    }
+}
+// (3) the weights 2^(s scale - m), their sum, and the weights times the tokens' norms as fp16.  The product in a fused multiply-add is
+// exact and m is one that was rounded: they differ by up to half a step of m, which is nothing below 2^20 but lets a weight
+// overflow where logits are beyond 2^31.  So rows with logits past 2^20 have their products rounded.  FAST: there are none, and every
+// row sees the whole tile; what a row gets does not depend on which of the two it goes through.
+template <int VB, bool FAST, class VNorm>
+__device__ __forceinline__ void weights(const float4_t (&s)[4], VNorm vn, int sees, float m, float scale, float &l, half8_t (&pf)[2]) {
+    const float off = FAST || m != -INFINITY ? m : 0.0f;
+    const bool near = fabsf(m) <= 0x1p20f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x = fmaf(s[u][i], scale, -off);
+            if constexpr (!FAST) {
+#pragma clang fp contract(off)
+                const float rounded = s[u][i] * scale - off;
+                x = near ? x : rounded;
+            }
+            const float w = __builtin_amdgcn_exp2f(x);
+            l += w;
+            float p = w;
+            if constexpr (VB != 8) {
+                p = w * vn(4 * u + i);
+                asm("" : "+v"(p));   // rounded to 32 bits before 16, FAST or not: the compiler makes one instruction with one rounding of some
+                if constexpr (!FAST) p = 4 * u + i < sees ? p : 0.0f;   // what a masked place holds may be no number
+            }
+            // int8 rows: the order 0, 2, 1, 3
+            const int to = VB == 8 ? ((i & 1) << 1) | (i >> 1) : i;
+            pf[u >> 1][4 * (u & 1) + to] = (_Float16)p;
+        }
+}
+// whether some row's logits are beyond what FAST weights are for
+template <int RB> __device__ __forceinline__ bool far_logits(const float (&m)[RB]) {
+    bool far = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) far = far || fabsf(m[rb]) > 0x1p20f;   // of -inf, too: nothing was seen so far
+    return __builtin_amdgcn_ballot_w64(far) != 0ull;
+}
+
+// What a walk leaves of a row block (o, m and the sum of weights over the row): the output, or this split's partial result
+template <int RB>
+__device__ __forceinline__ void leave_rows(const PagedAttnArgs &a, const PagedBlock &k, int first, int head, int split, int lane, const float4_t (&o)[RB][2][4],
+                                           const float (&m)[RB], const float (&l)[RB]) {
+    const int n16 = lane & 15, kq = lane >> 4;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
+        const int r = first + 16 * rb + n16;
+        const bool there = r < k.n_rows;
+        const int t = (int)a.group_div.div((uint32_t)(there ? r : 0)), hq = head * a.group + (there ? r : 0) - t * a.group;
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = o[rb][e >> 4][(e >> 2) & 3][e & 3];
+        if (k.span.splits <= 1) {
+            write_out(a, x, l[rb] > 0.0f ? a.v_unscale / l[rb] : l[rb] == 0.0f ? 0.0f : l[rb], k.seq.row0 + t, hq, there, lane);
+        } else if (there) {
+            const int64_t at = ((k.seq.row0 + t) * (a.r.p.n_kv_heads * a.group) + hq) * a.n_splits + split;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(a.part_o + at * 128 + out_dim(e, kq)) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+            if (kq == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * at) = make_float2(m[rb], l[rb]);
+        }
+    }
+}
+
+// This workgroup's KV head, split and number among the row blocks.  Neighbouring workgroups have the KV heads of the same rows:
+// with eight of them each die keeps to one head's pages.
+struct PagedTurn {
+    int head, split, turn;
+};
+__device__ __forceinline__ PagedTurn paged_turn(const PagedAttnArgs &a) {
+    const uint32_t rest = a.heads_div.div(blockIdx.x);
+    PagedTurn p;
+    p.head = (int)(blockIdx.x - rest * a.heads_div.d);
+    p.split = a.n_splits == 1 ? 0 : (int)(rest % (uint32_t)a.n_splits);
+    p.turn = a.n_splits == 1 ? (int)rest : (int)(rest / (uint32_t)a.n_splits);
+    return p;
+}
+
+// ---- 17 to 48 rows: every wavefront decodes for itself ---------------------------------------------------
+constexpr int ROWS_WAVES = 4;   // wavefronts of a workgroup
+// floats that a wavefront leaves behind for another one to join: 32 RB sums, RB maxima and sums of weights per lane
+__host__ __device__ constexpr int join_floats(int rb) { return 64 * 34 * rb; }
+__host__ __device__ constexpr int rows_copies(int bits) { return bits == 4 ? 16 : 32; }
+__host__ __device__ constexpr int rows_lds(int kb, int vb, int rb, bool share) {
+    const int tables = pair_table_bytes(kb, rows_copies(kb)) + (share ? 0 : pair_table_bytes(vb, rows_copies(vb))), join = ROWS_WAVES / 2 * join_floats(rb) * 4;
+    return tables > join ? tables : join;
+}
+
+// KB, VB: code widths, 8 for q8_0-style rows; RB: blocks of 16 rows per wavefront; SHARE: one table for K and V
+template <int KB, int VB, int RB, bool SHARE>
+__global__ __launch_bounds__(64 * ROWS_WAVES, RB == 2 ? 2 : 1) void k_paged_rows(PagedAttnArgs a) {
+    constexpr int W = ROWS_WAVES, TILE = 16 * RB;
+    constexpr int KBLOCK = KB == 8 ? TQ_ROWS_PER_BLOCK * 136 : block_bytes(KB), VBLOCK = VB == 8 ? TQ_ROWS_PER_BLOCK * 136 : block_bytes(VB);
+    __shared__ __attribute__((aligned(16))) char smem[rows_lds(KB, VB, RB, SHARE)];
+    __shared__ __attribute__((aligned(16))) uint4 q_s[W][RB][4][64];
+    __shared__ float scale_s[W][RB][64];
+    constexpr int KC = rows_copies(KB), VC = rows_copies(VB), V_TABLE = SHARE ? 0 : pair_table_bytes(KB, KC);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n16 = lane & 15, kq = lane >> 4;
+    const PagedTurn p = paged_turn(a);
+    const int head = p.head, split = p.split, kw = a.kw, part = wave & (kw - 1);
+    int b;
+    const PagedBlock rows = paged_block(a, p.turn * (W / kw) + wave / kw, TILE, split, b);
+    if (kw == W && !rows.active) return;    // all of the workgroup
+    int t_begin = 0, t_end = 0, least = 0;
+    if (rows.active) {
+        least = row_limit(a, rows, rows.r0);
+        t_begin = split * a.split_tiles;
+        t_end = min((row_limit(a, rows, min(rows.r0 + TILE, rows.n_rows) - 1) + 63) >> 6, t_begin + a.split_tiles);
+        const int each = (max(t_end - t_begin, 0) + kw - 1) / kw;
+        t_begin += part * each;
+        t_end = min(t_end, t_begin + each);
+    }
+    // ---- A tile's codes and norms are requested a tile ahead into the registers that its predecessor has just been read from: K's
+    // after the logits, V's after the values; the first one's before anything else.
+    const int32_t *table = a.r.p.block_table + (int64_t)__builtin_amdgcn_readfirstlane(b) * a.r.p.table_stride;
+    auto page_of = [&](int tile) { return scalar_entry(table, __builtin_amdgcn_readfirstlane(tile >> 1)); };
+    auto is_page = [&](int page) { return page >= 0 && page < a.r.p.n_pages; };
+    auto block_at = [&](int page) { return (int64_t)(is_page(page) ? page : 0) * a.r.p.n_kv_heads + head; };
+    uint32_t kw_[4][KB == 8 ? 8 : KB], vw[4][VB == 8 ? 8 : VB];
+    uint32_t kn[8], vn[VB == 8 ? 32 : 8];   // norms of the lane's 16 tokens; 8-bit K: a scale per unit, 8-bit V: [32-dim block] of them
+    const int k_row = 16 * (n16 >> 2) + (n16 & 3);
+    auto load_k = [&](int tile, int page) {
+        const uint8_t *kb = a.k + block_at(page) * KBLOCK;
+        const int half = tile & 1;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int row = 64 * half + k_row + 4 * u;
+            if constexpr (KB == 8) {
+                const uint4 lo = *reinterpret_cast<const uint4 *>(kb + (2 * kq) * 2048 + row * 16);
+                const uint4 hi = *reinterpret_cast<const uint4 *>(kb + (2 * kq + 1) * 2048 + row * 16);
+                kw_[u][0] = lo.x; kw_[u][1] = lo.y; kw_[u][2] = lo.z; kw_[u][3] = lo.w;
+                kw_[u][4] = hi.x; kw_[u][5] = hi.y; kw_[u][6] = hi.z; kw_[u][7] = hi.w;
+                kn[u] = reinterpret_cast<const uint16_t *>(kb + 8 * 2048)[4 * row + kq];
+            } else {
+#pragma unroll
+                for (int j = 0; j < KB; ++j) kw_[u][j] = *reinterpret_cast<const uint32_t *>(kb + j * 2048 + row * 16 + kq * 4);
+            }
+        }
+        if constexpr (KB != 8) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const uint4 n = *reinterpret_cast<const uint4 *>(kb + block_code_bytes(KB) + 2 * (64 * half + 16 * kq) + 16 * c);
+                kn[4 * c] = n.x; kn[4 * c + 1] = n.y; kn[4 * c + 2] = n.z; kn[4 * c + 3] = n.w;
+            }
+        }
+    };
+    auto load_v = [&](int tile, int page) {
+        const uint8_t *vb = a.v + block_at(page) * VBLOCK;
+        const int half = tile & 1;
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) {
+            const int row = 64 * half + 16 * blk + n16;
+            if constexpr (VB == 8) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(vb + (4 * hf + kq) * 2048 + row * 16);
+                    vw[blk][4 * hf] = w.x; vw[blk][4 * hf + 1] = w.y; vw[blk][4 * hf + 2] = w.z; vw[blk][4 * hf + 3] = w.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VB; ++j) vw[blk][j] = *reinterpret_cast<const uint32_t *>(vb + j * 2048 + row * 16 + kq * 4);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < (VB == 8 ? 8 : 2); ++c) {
+            const uint8_t *side = VB == 8 ? vb + 8 * 2048 + 2 * ((half * 4 + (c >> 1)) * 64 + 16 * kq) + 16 * (c & 1)
+                                          : vb + 128 * 16 * VB + 2 * (64 * half + 16 * kq) + 16 * c;
+            const uint4 n = *reinterpret_cast<const uint4 *>(side);
+            vn[4 * c] = n.x; vn[4 * c + 1] = n.y; vn[4 * c + 2] = n.z; vn[4 * c + 3] = n.w;
+        }
+    };
+
+    int page = 0, page_next = 0;
+    if (t_begin < t_end) {
+        page = page_of(t_begin);
+        page_next = page_of(min(t_begin + 1, t_end - 1));
+        load_k(t_begin, page);
+        load_v(t_begin, page);
+    }
+    // queries: rotated by one wavefront of those that share the rows
+    if (part == 0) {
+        half8_t q0[RB][4];
+        float s0[RB];
+        int n0[RB];
+        load_queries<KB, RB>(a, rows, rows.r0, head, lane, q0, s0, n0);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) q_s[wave / kw][rb][ks][lane] = __builtin_bit_cast(uint4, q0[rb][ks]);
+            scale_s[wave / kw][rb][lane] = s0[rb];
+        }
+    }
+    if constexpr (KB != 8) build_pair_table<KB, KC>(smem, a.klut, tid, 64 * W);
+    if constexpr (VB != 8 && !SHARE) build_pair_table<VB, VC>(smem + V_TABLE, a.vlut, tid, 64 * W);
+    const uint32_t k_copy = 4 * (lane & (KC - 1)), v_copy = 4 * (lane & (VC - 1));
+    __syncthreads();   // the tables and the queries
+    half8_t qf[RB][4];
+    float scale[RB], m[RB], l[RB];
+    int seen[RB];
+    float4_t o[RB][2][4];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) qf[rb][ks] = __builtin_bit_cast(half8_t, q_s[wave / kw][rb][ks][lane]);
+        scale[rb] = scale_s[wave / kw][rb][lane];
+        seen[rb] = row_limit(a, rows, min(rows.r0 + 16 * rb + n16, max(rows.n_rows - 1, 0)));
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[rb][e >> 2][e & 3] = float4_t{0.f, 0.f, 0.f, 0.f};
         m[rb] = -INFINITY;
         l[rb] = 0.0f;
     }
-    __syncthreads();   // the tables
 
-    const int32_t *table = a.r.p.block_table + (int64_t)b * a.r.p.table_stride;
-    auto page_of = [&](int tile) { return __builtin_amdgcn_readfirstlane(table[tile >> 1]); };
-    int page = t_begin < t_end ? page_of(t_begin) : 0;
-#pragma unroll 1
-    for (int tile = t_begin; tile < t_end; ++tile) {
-        const bool real = page >= 0 && page < a.r.p.n_pages;
-        const int64_t at = (int64_t)(real ? page : 0) * a.r.p.n_kv_heads + head;
-        const uint8_t *kb = a.k + at * KBLOCK, *vb = a.v + at * VBLOCK;
-        const int half = tile & 1, first = 64 * tile + 16 * kq;     // this lane's tokens: first + 4 u + i
-        if (tile + 1 < t_end) page = page_of(tile + 1);
-        const bool masked = !real || 64 * tile + 64 > least;   // some row does not see all of the tile
+    // one tile; masked_t: some row does not see all of it, or its page is none
+    auto do_tile = [&](auto masked_t, int tile, bool real, int page_next) {
+        constexpr bool MASKED = decltype(masked_t)::value;
+        const int first = 64 * tile + 16 * kq;     // this lane's tokens: first + 4 u + i
+        const int next = min(tile + 1, t_end - 1);
         // ---- logits
         float4_t s[RB][4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int row = 64 * half + 16 * (n16 >> 2) + 4 * u + (n16 & 3);
             half8_t kf[4];
             if constexpr (KB == 8) {
-                const uint4 lo = *reinterpret_cast<const uint4 *>(kb + (2 * kq) * 2048 + row * 16);
-                const uint4 hi = *reinterpret_cast<const uint4 *>(kb + (2 * kq + 1) * 2048 + row * 16);
-                const _Float16 d = reinterpret_cast<const _Float16 *>(kb + 8 * 2048)[4 * row + kq];
+                const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)kn[u]);
                 const half2_t dd = {d, d};
-                kf[0] = join(int8x4_times(lo.x, dd, dd), int8x4_times(lo.y, dd, dd));
-                kf[1] = join(int8x4_times(lo.z, dd, dd), int8x4_times(lo.w, dd, dd));
-                kf[2] = join(int8x4_times(hi.x, dd, dd), int8x4_times(hi.y, dd, dd));
-                kf[3] = join(int8x4_times(hi.z, dd, dd), int8x4_times(hi.w, dd, dd));
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) kf[ks] = join(int8x4_times(kw_[u][2 * ks], dd, dd), int8x4_times(kw_[u][2 * ks + 1], dd, dd));
             } else {
-                uint32_t w[KB];
+                const uint32_t tail = group_tail<KB>(kw_[u]);
 #pragma unroll
-                for (int j = 0; j < KB; ++j) w[j] = *reinterpret_cast<const uint32_t *>(kb + j * 2048 + row * 16 + kq * 4);
-                const uint32_t tail = group_tail<KB>(w);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) kf[ks] = join(group_quad<KB>(w, tail, klut, 2 * ks), group_quad<KB>(w, tail, klut, 2 * ks + 1));
+                for (int ks = 0; ks < 4; ++ks) kf[ks] = join(group_quad<KB, KC>(kw_[u], tail, smem, k_copy, 2 * ks), group_quad<KB, KC>(kw_[u], tail, smem, k_copy, 2 * ks + 1));
             }
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
@@ -323,88 +538,44 @@ __global__ __launch_bounds__(64 * paged_waves(RB)) void k_paged_attn(PagedAttnAr
                 for (int ks = 0; ks < 4; ++ks) s[rb][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[ks], qf[rb][ks], s[rb][u], 0, 0, 0);
             }
         }
-        // the tokens' norms; 0 where the page is none, so that nothing it may hold gets in
-        uint32_t kn[8], vn[8];
+        float knf[16];
+        if constexpr (KB != 8) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if constexpr (KB != 8) {
-                const uint4 n = *reinterpret_cast<const uint4 *>(kb + block_code_bytes(KB) + 2 * (64 * half + 16 * kq) + 16 * c);
-                kn[4 * c] = n.x; kn[4 * c + 1] = n.y; kn[4 * c + 2] = n.z; kn[4 * c + 3] = n.w;
-            }
-            if constexpr (VB != 8) {
-                const uint4 n = *reinterpret_cast<const uint4 *>(vb + block_code_bytes(VB) + 2 * (64 * half + 16 * kq) + 16 * c);
-                vn[4 * c] = n.x; vn[4 * c + 1] = n.y; vn[4 * c + 2] = n.z; vn[4 * c + 3] = n.w;
-            }
+            for (int e = 0; e < 16; ++e) knf[e] = half_of(kn[e >> 1], e & 1);
         }
+        load_k(next, page_next);
+        __builtin_amdgcn_sched_barrier(0);   // the scheduler otherwise has all look-ups in flight and spills
         // ---- softmax
         half8_t pf[RB][2];
+        float m_new[RB];
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            float most = -INFINITY;
-            const int sees = real ? seen[rb] - first : 0;    // this lane's tokens 0 .. sees - 1 count
+        for (int rb = 0; rb < RB; ++rb)
+            m_new[rb] = logits_max<KB, MASKED>(s[rb], [&](int e) { return knf[e]; }, real ? seen[rb] - first : 0, scale[rb], m[rb]);
+        move_max<RB>(m_new, m, l, o);
+        auto all_weights = [&](auto fast_t) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = s[rb][u][i];
-                    if constexpr (KB != 8) v *= half_of(kn[2 * u + (i >> 1)], i & 1);
-                    if (masked) v = 4 * u + i < sees ? v : -INFINITY;
-                    s[rb][u][i] = v;
-                    most = fmaxf(most, v);
-                }
-            const float m_new = fmaxf(m[rb], over_row_max(most) * scale[rb]);
-            if (__builtin_amdgcn_ballot_w64(m_new != m[rb]) != 0ull) {
-                const float shrink = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rb] - m_new);
-                l[rb] *= shrink;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[rb][e >> 2][e & 3] *= shrink;
-                m[rb] = m_new;
-            }
-            float off = m[rb] == -INFINITY ? 0.0f : m[rb], by = scale[rb];
-            // The product in a fused multiply-add is exact and m is one that was rounded: they differ by up to half a step of m, which
-            // is nothing below 2^20 but lets a weight overflow where logits are beyond 2^31.
-            if (__builtin_amdgcn_ballot_w64(fabsf(off) > 0x1p20f) != 0ull) {
-#pragma clang fp contract(off)
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[rb][u][i] = s[rb][u][i] * by - off;
-                off = 0.0f;
-                by = 1.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(s[rb][u][i], by, -off));
-                    l[rb] += w;
-                    float p = w;
-                    if constexpr (VB != 8) {
-                        p *= half_of(vn[2 * u + (i >> 1)], i & 1);
-                        if (masked) p = 4 * u + i < sees ? p : 0.0f;   // what a masked place holds may be no number
-                    }
-                    // int8 rows: the order 0, 2, 1, 3
-                    const int to = VB == 8 ? ((i & 1) << 1) | (i >> 1) : i;
-                    pf[rb][u >> 1][4 * (u & 1) + to] = (_Float16)p;
-                }
-        }
+            for (int rb = 0; rb < RB; ++rb)
+                weights<VB, decltype(fast_t)::value>(s[rb], [&](int e) { return half_of(vn[e >> 1], e & 1); }, real ? seen[rb] - first : 0, m[rb], scale[rb],
+                                                     l[rb], pf[rb]);
+        };
+        if constexpr (MASKED) all_weights(std::false_type{});
+        else if (far_logits<RB>(m)) all_weights(std::false_type{});
+        else all_weights(std::true_type{});
+        __builtin_amdgcn_sched_barrier(0);
         // ---- values
 #pragma unroll
         for (int blk = 0; blk < 4; ++blk) {
-            const int row = 64 * half + 16 * blk + n16;
             half8_t vf[2][2];   // [dims' half][step]
             if constexpr (VB == 8) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(vb + (4 * hf + kq) * 2048 + row * 16);
-                    const uint4 *d4 = reinterpret_cast<const uint4 *>(vb + 8 * 2048 + 2 * ((half * 4 + 2 * hf + (blk >> 1)) * 64 + 16 * kq));
-                    const uint4 d0 = d4[0], d1 = d4[1];
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-                    uint32_t d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+                    uint32_t d[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) d[j] = vn[8 * (2 * hf + (blk >> 1)) + j];
                     // In a tile that some row does not see whole, a scale that is no finite number (of rows that held none, or of a
                     // place that nothing was written to) must not reach the rows that do not see its token, and 0 times
                     // it would: it is replaced, and the rows that see it are marked.
-                    if (masked) {
+                    if constexpr (MASKED) {
                         uint32_t bad = 0;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -425,21 +596,18 @@ __global__ __launch_bounds__(64 * paged_waves(RB)) void k_paged_attn(PagedAttnAr
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         const uint32_t d02 = __builtin_amdgcn_perm(d[2 * u + 1], d[2 * u], 0x05040100u), d13 = __builtin_amdgcn_perm(d[2 * u + 1], d[2 * u], 0x07060302u);
-                        q4[u] = int8x4_times(ww[u], __builtin_bit_cast(half2_t, d02), __builtin_bit_cast(half2_t, d13));
+                        q4[u] = int8x4_times(vw[blk][4 * hf + u], __builtin_bit_cast(half2_t, d02), __builtin_bit_cast(half2_t, d13));
                     }
                     vf[hf][0] = join(q4[0], q4[1]);
                     vf[hf][1] = join(q4[2], q4[3]);
                 }
             } else {
-                uint32_t w[VB];
-#pragma unroll
-                for (int j = 0; j < VB; ++j) w[j] = *reinterpret_cast<const uint32_t *>(vb + j * 2048 + row * 16 + kq * 4);
-                const uint32_t tail = group_tail<VB>(w);
+                const uint32_t tail = group_tail<VB>(vw[blk]);
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                     for (int st = 0; st < 2; ++st)
-                        vf[hf][st] = join(group_quad<VB>(w, tail, vlut, 4 * st + hf), group_quad<VB>(w, tail, vlut, 4 * st + 2 + hf));
+                        vf[hf][st] = join(group_quad<VB, VC>(vw[blk], tail, smem + V_TABLE, v_copy, 4 * st + hf), group_quad<VB, VC>(vw[blk], tail, smem + V_TABLE, v_copy, 4 * st + 2 + hf));
             }
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
@@ -448,6 +616,26 @@ __global__ __launch_bounds__(64 * paged_waves(RB)) void k_paged_attn(PagedAttnAr
 #pragma unroll
                     for (int st = 0; st < 2; ++st)
                         o[rb][hf][blk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[hf][st], pf[rb][st], o[rb][hf][blk], 0, 0, 0);
+        }
+        load_v(next, page_next);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (t_begin < t_end) {
+        const int whole = min(max(least >> 6, t_begin), t_end);     // tiles that every row sees
+        int tile = t_begin;
+#pragma unroll 1
+        for (; tile < whole && is_page(page); ++tile) {
+            const int after = page_of(min(tile + 2, t_end - 1));
+            do_tile(std::false_type{}, tile, true, page_next);
+            page = page_next;
+            page_next = after;
+        }
+#pragma unroll 1
+        for (; tile < t_end; ++tile) {
+            const int after = page_of(min(tile + 2, t_end - 1));
+            do_tile(std::true_type{}, tile, is_page(page), page_next);
+            page = page_next;
+            page_next = after;
         }
     }
 #pragma unroll
@@ -485,24 +673,295 @@ __global__ __launch_bounds__(64 * paged_waves(RB)) void k_paged_attn(PagedAttnAr
             }
         }
     }
-    if (part != 0 || !active) return;
+    if (part == 0 && rows.active) leave_rows<RB>(a, rows, rows.r0, head, split, lane, o, m, l);
+}
+
+// ---- many rows: a workgroup decodes a tile once for all of its wavefronts ------------------------------------
+// 32 rows per wavefront, 32 W per workgroup.  Every tile's operands are decoded by the wavefronts in turns of a 16-token unit of K or
+// a 16-dim block of V and lie in LDS as the matrix instructions take them (a lane's 16 bytes next to its neighbour's), a tile ahead
+// of their use, behind one barrier per tile.
+// copies of a decode table: a workgroup looks each pair up once, and two of its size share a CU's LDS
+__host__ __device__ constexpr int chunk_copies(int bits) { return bits == 4 ? 4 : 16; }
+template <int KB, int VB, int W, int RB>
+__global__ __launch_bounds__(64 * W, 2) void k_paged_chunk(PagedAttnArgs a) {
+    constexpr int TILE = 16 * RB * W, KC = chunk_copies(KB), VC = chunk_copies(VB);
+    constexpr int KBLOCK = KB == 8 ? TQ_ROWS_PER_BLOCK * 136 : block_bytes(KB), VBLOCK = VB == 8 ? TQ_ROWS_PER_BLOCK * 136 : block_bytes(VB);
+    __shared__ __attribute__((aligned(16))) uint4 kf_s[2][4][4][64], vf_s[2][4][4][64];   // [buffer][unit][step], [block][half of the dims, step]
+    __shared__ __attribute__((aligned(16))) char lut_s[pair_table_bytes(KB, KC) + pair_table_bytes(VB, VC) + 16];
+    __shared__ __attribute__((aligned(16))) float kn_s[2][64], vn_s[2][64];
+    __shared__ uint32_t bad_s[2][16];     // 8-bit V: [32-dim block][quarter]: tokens whose scale is no finite number
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n16 = lane & 15, kq = lane >> 4;
+    const PagedTurn p = paged_turn(a);
+    const int head = p.head, split = p.split;
+    int b;
+    const PagedBlock rows = paged_block(a, p.turn, TILE, split, b);
+    if (!rows.active) return;    // all of the workgroup
+    const int first_row = rows.r0 + 16 * RB * wave;
+    const bool computes = first_row < rows.n_rows;
+    const int t_begin = split * a.split_tiles;
+    const int t_end = min((row_limit(a, rows, min(rows.r0 + TILE, rows.n_rows) - 1) + 63) >> 6, t_begin + a.split_tiles);
+    // of this wavefront's rows: the tiles that all of them see, and those that any does
+    const int whole = computes ? min(t_end, row_limit(a, rows, first_row) >> 6) : 0;
+    const int upto = computes ? min(t_end, (row_limit(a, rows, min(first_row + 16 * RB, rows.n_rows) - 1) + 63) >> 6) : 0;
+
+    // ---- decoding: wavefronts 0 .. 3 have K units, the last four (W = 4: the same ones) V blocks
+    constexpr bool BOTH = W == 4;
+    const int32_t *table = a.r.p.block_table + (int64_t)__builtin_amdgcn_readfirstlane(b) * a.r.p.table_stride;
+    auto page_of = [&](int tile) { return scalar_entry(table, __builtin_amdgcn_readfirstlane(min(tile, t_end - 1) >> 1)); };
+    auto is_page = [&](int page) { return page >= 0 && page < a.r.p.n_pages; };
+    const bool does_k = BOTH || wave < 4, does_v = BOTH || wave >= 4;
+    const int unit = wave & 3, k_token = 16 * (n16 >> 2) + 4 * unit + (n16 & 3), v_row = 16 * unit + n16;
+    uint32_t kw[KB == 8 ? 8 : KB], vw[VB == 8 ? 8 : VB], vsc[VB == 8 ? 16 : 1];
+    uint16_t kn = 0, vn = 0;
+    auto request_k = [&](int tile, int page) __attribute__((always_inline)) {
+        const uint8_t *kb = a.k + ((int64_t)(is_page(page) ? page : 0) * a.r.p.n_kv_heads + head) * KBLOCK;
+        const int base = 64 * (min(tile, t_end - 1) & 1);
+        if (does_k) {
+            const int row = base + k_token;
+            if constexpr (KB == 8) {
+                const uint4 lo = *reinterpret_cast<const uint4 *>(kb + (2 * kq) * 2048 + row * 16), hi = *reinterpret_cast<const uint4 *>(kb + (2 * kq + 1) * 2048 + row * 16);
+                kw[0] = lo.x; kw[1] = lo.y; kw[2] = lo.z; kw[3] = lo.w;
+                kw[4] = hi.x; kw[5] = hi.y; kw[6] = hi.z; kw[7] = hi.w;
+                kn = reinterpret_cast<const uint16_t *>(kb + 8 * 2048)[4 * row + kq];
+            } else {
+#pragma unroll
+                for (int j = 0; j < KB; ++j) kw[j] = *reinterpret_cast<const uint32_t *>(kb + j * 2048 + row * 16 + kq * 4);
+                kn = reinterpret_cast<const uint16_t *>(kb + block_code_bytes(KB))[row];
+            }
+        }
+    };
+    auto request_v = [&](int tile, int page) __attribute__((always_inline)) {
+        const uint8_t *vb = a.v + ((int64_t)(is_page(page) ? page : 0) * a.r.p.n_kv_heads + head) * VBLOCK;
+        const int base = 64 * (min(tile, t_end - 1) & 1);
+        if (does_v) {
+            const int row = base + v_row;
+            if constexpr (VB == 8) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(vb + (4 * hf + kq) * 2048 + row * 16);
+                    vw[4 * hf] = w.x; vw[4 * hf + 1] = w.y; vw[4 * hf + 2] = w.z; vw[4 * hf + 3] = w.w;
+                    const uint4 *d = reinterpret_cast<const uint4 *>(vb + 8 * 2048 + 2 * ((4 * (base >> 6) + 2 * hf + (unit >> 1)) * 64 + 16 * kq));
+                    const uint4 d0 = d[0], d1 = d[1];
+                    vsc[8 * hf] = d0.x; vsc[8 * hf + 1] = d0.y; vsc[8 * hf + 2] = d0.z; vsc[8 * hf + 3] = d0.w;
+                    vsc[8 * hf + 4] = d1.x; vsc[8 * hf + 5] = d1.y; vsc[8 * hf + 6] = d1.z; vsc[8 * hf + 7] = d1.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VB; ++j) vw[j] = *reinterpret_cast<const uint32_t *>(vb + j * 2048 + row * 16 + kq * 4);
+                vn = reinterpret_cast<const uint16_t *>(vb + block_code_bytes(VB))[row];   // of token 16 unit + n16
+            }
+        }
+    };
+    const char *vlut = lut_s + (a.share ? 0 : pair_table_bytes(KB, KC));
+    const uint32_t k_copy = 4 * (lane & (KC - 1)), v_copy = 4 * (lane & (VC - 1));
+    auto decode_k = [&](int buf) __attribute__((always_inline)) {
+        if (does_k) {
+            if constexpr (KB == 8) {
+                const _Float16 d = __builtin_bit_cast(_Float16, kn);
+                const half2_t dd = {d, d};
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    kf_s[buf][unit][ks][lane] = __builtin_bit_cast(uint4, join(int8x4_times(kw[2 * ks], dd, dd), int8x4_times(kw[2 * ks + 1], dd, dd)));
+            } else {
+                const uint32_t tail = group_tail<KB>(kw);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    kf_s[buf][unit][ks][lane] = make_uint4(group_pair<KB, KC>(kw, tail, lut_s, k_copy, 4 * ks), group_pair<KB, KC>(kw, tail, lut_s, k_copy, 4 * ks + 1),
+                                                           group_pair<KB, KC>(kw, tail, lut_s, k_copy, 4 * ks + 2), group_pair<KB, KC>(kw, tail, lut_s, k_copy, 4 * ks + 3));
+                if (kq == 0) kn_s[buf][k_token] = __half2float(__ushort_as_half(kn));
+            }
+        }
+    };
+    auto decode_v = [&](int buf) __attribute__((always_inline)) {
+        if (does_v) {
+            if constexpr (VB == 8) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    // a scale that is no finite number would reach rows that do not see its token, as 0 times it: it is replaced, and the
+                    // rows that see it are marked
+                    uint32_t d[8], bad = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        d[j] = vsc[8 * hf + j];
+                        const bool lo = (d[j] & 0x7C00u) == 0x7C00u, hi = (d[j] & 0x7C000000u) == 0x7C000000u;
+                        bad |= (lo ? 1u << (2 * j) : 0u) | (hi ? 2u << (2 * j) : 0u);
+                        d[j] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+                    }
+                    if ((unit & 1) == 0 && n16 == 0) bad_s[buf][4 * (2 * hf + (unit >> 1)) + kq] = bad;
+                    uint2 q4[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t d02 = __builtin_amdgcn_perm(d[2 * u + 1], d[2 * u], 0x05040100u), d13 = __builtin_amdgcn_perm(d[2 * u + 1], d[2 * u], 0x07060302u);
+                        q4[u] = int8x4_times(vw[4 * hf + u], __builtin_bit_cast(half2_t, d02), __builtin_bit_cast(half2_t, d13));
+                    }
+                    vf_s[buf][unit][2 * hf][lane] = __builtin_bit_cast(uint4, join(q4[0], q4[1]));
+                    vf_s[buf][unit][2 * hf + 1][lane] = __builtin_bit_cast(uint4, join(q4[2], q4[3]));
+                }
+            } else {
+                const uint32_t tail = group_tail<VB>(vw);
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        const int p0 = 2 * (4 * st + hf);   // quads 4 st + hf and two further
+                        vf_s[buf][unit][2 * hf + st][lane] = make_uint4(group_pair<VB, VC>(vw, tail, vlut, v_copy, p0), group_pair<VB, VC>(vw, tail, vlut, v_copy, p0 + 1),
+                                                                        group_pair<VB, VC>(vw, tail, vlut, v_copy, p0 + 4), group_pair<VB, VC>(vw, tail, vlut, v_copy, p0 + 5));
+                    }
+                if (kq == 0) vn_s[buf][v_row] = __half2float(__ushort_as_half(vn));
+            }
+        }
+    };
+
+    int page = 0, page1 = 0, page2 = 0;    // of this tile and the next two
+    if (t_begin < t_end) {
+        page = page_of(t_begin);
+        page1 = page_of(t_begin + 1);
+        page2 = page_of(t_begin + 2);
+        request_k(t_begin, page);
+        request_v(t_begin, page);
+    }
+    if constexpr (KB != 8) build_pair_table<KB, KC>(lut_s, a.klut, tid, 64 * W);
+    if constexpr (VB != 8)
+        if (!a.share) build_pair_table<VB, VC>(lut_s + pair_table_bytes(KB, KC), a.vlut, tid, 64 * W);
+    half8_t qf[RB][4];
+    float scale[RB], m[RB], l[RB];
+    int seen[RB];
+    load_queries<KB, RB>(a, rows, first_row, head, lane, qf, scale, seen);
+    float4_t o[RB][2][4];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        const int r = r0 + 16 * rb + n16;
-        const bool there = r < n_rows;
-        const int t = (int)a.group_div.div((uint32_t)(there ? r : 0)), hq = head * a.group + (there ? r : 0) - t * a.group;
-        float x[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = o[rb][e >> 4][(e >> 2) & 3][e & 3];
-        if (span.splits <= 1) {
-            write_out(a, x, l[rb] > 0.0f ? a.v_unscale / l[rb] : l[rb] == 0.0f ? 0.0f : l[rb], seq.row0 + t, hq, there, lane);
-        } else if (there) {
-            const int64_t at = ((seq.row0 + t) * (a.r.p.n_kv_heads * a.group) + hq) * a.n_splits + split;
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(a.part_o + at * 128 + out_dim(e, kq)) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-            if (kq == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * at) = make_float2(m[rb], l[rb]);
-        }
+        for (int e = 0; e < 8; ++e) o[rb][e >> 2][e & 3] = float4_t{0.f, 0.f, 0.f, 0.f};
+        m[rb] = -INFINITY;
+        l[rb] = 0.0f;
     }
+    __syncthreads();   // the tables
+    // The logits of the next tile are multiplied while this one's weights are worked out, and the next one's maximum is found while
+    // this one's values are multiplied: K is decoded two tiles ahead, V one.
+    if (t_begin < t_end) {
+        decode_k(t_begin & 1);
+        decode_v(t_begin & 1);
+        request_k(t_begin + 1, page1);
+        request_v(t_begin + 1, page1);
+        decode_k((t_begin + 1) & 1);
+        request_k(t_begin + 2, page2);
+    }
+    __syncthreads();
+
+    auto logits = [&](int tile, float4_t (&s)[RB][4]) __attribute__((always_inline)) {
+        const int buf = tile & 1;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) s[rb][u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                const half8_t kf = __builtin_bit_cast(half8_t, kf_s[buf][u][ks][lane]);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) s[rb][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rb][ks], s[rb][u], 0, 0, 0);
+            }
+        }
+    };
+    float m_new[RB];
+    auto maxima = [&](auto fast_t, int tile, bool real, float4_t (&s)[RB][4]) __attribute__((always_inline)) {
+        constexpr bool FAST = decltype(fast_t)::value;
+        const int buf = tile & 1, first = 64 * tile + 16 * kq;     // this lane's tokens: first + 4 u + i
+        float4_t knf[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if constexpr (KB != 8) knf[u] = *reinterpret_cast<const float4_t *>(&kn_s[buf][16 * kq + 4 * u]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+            m_new[rb] = logits_max<KB, !FAST>(s[rb], [&](int e) { return knf[e >> 2][e & 3]; }, real ? seen[rb] - first : 0, scale[rb], m[rb]);
+    };
+    auto values = [&](int tile, const half8_t (&pf)[RB][2]) __attribute__((always_inline)) {
+        const int buf = tile & 1;
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const half8_t vf = __builtin_bit_cast(half8_t, vf_s[buf][blk][2 * hf + st][lane]);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) o[rb][hf][blk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rb][st], o[rb][hf][blk], 0, 0, 0);
+                }
+    };
+    auto all_weights = [&](auto fast_t, int tile, bool real, const float4_t (&s)[RB][4], half8_t (&pf)[RB][2]) __attribute__((always_inline)) {
+        constexpr bool FAST = decltype(fast_t)::value;
+        const int buf = tile & 1, first = 64 * tile + 16 * kq;
+        float4_t vnf[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if constexpr (VB != 8) vnf[u] = *reinterpret_cast<const float4_t *>(&vn_s[buf][16 * kq + 4 * u]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+            weights<VB, FAST>(s[rb], [&](int e) { return vnf[e >> 2][e & 3]; }, real ? seen[rb] - first : 0, m[rb], scale[rb], l[rb], pf[rb]);
+        if constexpr (VB == 8) {
+            const uint32_t bad = bad_s[buf][n16];
+            if (__builtin_amdgcn_ballot_w64(bad != 0u) != 0ull) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t mine = bad_s[buf][4 * j + kq];
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        const int sees = real ? min(max(seen[rb] - first, 0), 16) : 0;
+                        if (over_row_max((mine & ((1u << sees) - 1u)) ? 1.0f : 0.0f) > 0.0f)
+                            o[rb][j >> 1][2 * (j & 1)] = o[rb][j >> 1][2 * (j & 1) + 1] = float4_t{NAN, NAN, NAN, NAN};
+                    }
+                }
+            }
+        }
+    };
+    auto decode_next = [&](int tile) __attribute__((always_inline)) {
+        decode_v((tile + 1) & 1);
+        decode_k(tile & 1);
+        page = page1;
+        page1 = page2;
+        page2 = page_of(tile + 3);
+        request_v(tile + 2, page1);
+        request_k(tile + 3, page2);
+        __syncthreads();
+    };
+    float4_t s[RB][4];     // this tile's logits, with norms and masks
+    if (upto > t_begin) {
+        logits(t_begin, s);
+        maxima(std::false_type{}, t_begin, is_page(page), s);
+    }
+    __syncthreads();
+    int tile = t_begin;
+#pragma unroll 1
+    for (; tile + 1 < whole && is_page(page) && is_page(page1) && !far_logits<RB>(m_new); ++tile) {
+        move_max<RB>(m_new, m, l, o);
+        float4_t next[RB][4];
+        half8_t pf[RB][2];
+        logits(tile + 1, next);
+        all_weights(std::true_type{}, tile, true, s, pf);
+        values(tile, pf);
+        maxima(std::true_type{}, tile + 1, true, next);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[rb][u] = next[rb][u];
+        decode_next(tile);
+    }
+#pragma unroll 1
+    for (; tile < t_end; ++tile) {
+        if (tile < upto) {
+            half8_t pf[RB][2];
+            move_max<RB>(m_new, m, l, o);
+            all_weights(std::false_type{}, tile, is_page(page), s, pf);
+            values(tile, pf);
+            logits(tile + 1, s);
+            maxima(std::false_type{}, tile + 1, is_page(page1), s);
+        }
+        decode_next(tile);
+    }
+    if (!computes) return;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) l[rb] = over_row_sum(l[rb]);
+    leave_rows<RB>(a, rows, first_row, head, split, lane, o, m, l);
 }
 
 }  // namespace tqpaged

@@ -1,27 +1,34 @@
-// The kernels of one K width, by V's width, shared table and row blocks.
+// The kernels of one K width, by V's width and the number of rows.
 #pragma once
 #include "tq_paged_attn.h"
 
 namespace tqpaged {
 
-template <int KB, int VB, bool SHARE> int launch_rows(const PagedAttnArgs &a, int rb, unsigned grid, hipStream_t s) {
-    switch (rb) {
-    case 1: k_paged_attn<KB, VB, 1, SHARE><<<grid, 64 * paged_waves(1), 0, s>>>(a); break;
-    case 2: k_paged_attn<KB, VB, 2, SHARE><<<grid, 64 * paged_waves(2), 0, s>>>(a); break;
-    default: k_paged_attn<KB, VB, 4, SHARE><<<grid, 64 * paged_waves(4), 0, s>>>(a); break;
+template <int KB, int VB, int RB> void launch_rows(const PagedAttnArgs &a, unsigned grid, hipStream_t s) {
+    if constexpr (KB == VB && KB != 8) {
+        if (a.share) {
+            k_paged_rows<KB, VB, RB, true><<<grid, 64 * ROWS_WAVES, 0, s>>>(a);
+            return;
+        }
+    }
+    k_paged_rows<KB, VB, RB, false><<<grid, 64 * ROWS_WAVES, 0, s>>>(a);
+}
+template <int KB, int VB> int launch_kind(const PagedAttnArgs &a, PagedKind kind, unsigned grid, hipStream_t s) {
+    switch (kind) {
+    case ROWS_32: launch_rows<KB, VB, 2>(a, grid, s); break;
+    case ROWS_48: launch_rows<KB, VB, 3>(a, grid, s); break;
+    case CHUNK_128: k_paged_chunk<KB, VB, 4, 2><<<grid, 256, 0, s>>>(a); break;
+    default: k_paged_chunk<KB, VB, 8, 2><<<grid, 512, 0, s>>>(a); break;
     }
     return tq_check_launch("paged_attn");
 }
 
-template <int KB> int launch_k(const PagedAttnArgs &a, int vb, bool share, int rb, unsigned grid, hipStream_t s) {
-    if constexpr (KB != 8) {
-        if (share && vb == KB) return launch_rows<KB, KB, true>(a, rb, grid, s);
-    }
+template <int KB> int launch_k(const PagedAttnArgs &a, int vb, PagedKind kind, unsigned grid, hipStream_t s) {
     switch (vb) {
-    case 2: return launch_rows<KB, 2, false>(a, rb, grid, s);
-    case 3: return launch_rows<KB, 3, false>(a, rb, grid, s);
-    case 4: return launch_rows<KB, 4, false>(a, rb, grid, s);
-    default: return launch_rows<KB, 8, false>(a, rb, grid, s);
+    case 2: return launch_kind<KB, 2>(a, kind, grid, s);
+    case 3: return launch_kind<KB, 3>(a, kind, grid, s);
+    case 4: return launch_kind<KB, 4>(a, kind, grid, s);
+    default: return launch_kind<KB, 8>(a, kind, grid, s);
     }
 }
 

@@ -129,8 +129,8 @@ class PagedAttention:
     """softmax(scale q k^T) v of new tokens over a paged cache (tq_paged_attention): single tokens, a few drafted ones, chunks
     and whole prompts of a ragged batch, and (causal=False) queries over another sequence's states.
 
-    Holds a workspace that grows to the largest call's need: calls of one object must not overlap in time, captured ones
-    among them (an object per graph, or one workspace size from a first eager call, and replays in order).
+    Holds a workspace that grows to the largest call's need (a smaller one stays with the object, for calls that were captured with
+    it): calls of one object must not overlap in time, replayed ones among them.
     A codec of None stands for q8_0-style rows on that side.
     """
 
@@ -141,7 +141,7 @@ class PagedAttention:
         self.k_codec, self.v_codec = k_codec, v_codec
         self.n_q_heads, self.n_kv_heads, self.causal = n_q_heads, n_kv_heads, bool(causal)
         self.scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-        self.workspace = None
+        self.workspace, self._outgrown = None, []
 
     def __call__(self, q, k_pages, v_pages, block_table, lens, cu_new=None, *, max_context: int | None = None, max_new: int | None = None,
                  out=None):
@@ -172,6 +172,8 @@ class PagedAttention:
         if need < 0:
             L.check(L.ERR_ARG)
         if self.workspace is None or self.workspace.numel() < need or self.workspace.get_device() != device:
+            if self.workspace is not None:
+                self._outgrown.append(self.workspace)     # a captured call may still write to it
             self.workspace = tt.empty(need, dtype=tt.uint8, device=q.device)
         L.check(L.lib().tq_paged_attention(_handle(self.k_codec), _handle(self.v_codec), C.byref(p), q.data_ptr(), k_pages.data_ptr(),
                                            v_pages.data_ptr(), out.data_ptr(), self.workspace.data_ptr(), self.workspace.numel(),
