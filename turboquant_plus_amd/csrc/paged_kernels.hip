@@ -26,11 +26,11 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedAttnArgs a) 
     const int head = (int)(at - row * heads);
     if (row >= a.r.rows) return;
     int b, nth;
-    if (!paged_item(a.r, (int)row, [&](int s) { return paged_seq(a.r, s).n; }, b, nth)) return;
-    const PagedSeq seq = paged_seq(a.r, b);
+    PagedSeq seq;
+    if (!paged_item(a.r, (int)row, [&](const PagedSeq &q) { return q.n; }, b, nth, seq)) return;
     const PagedSpan span = paged_span(a, seq);
     if (span.splits <= 1 || nth >= a.max_new) return;
-    const int64_t place = ((seq.row0 + nth) * heads + head) * a.n_splits;
+    const int64_t place = ((int64_t)(seq.row0 + nth) * heads + head) * a.n_splits;
     float top = -INFINITY;
     for (int s = lane; s < span.splits; s += 64) top = fmaxf(top, a.part_ml[2 * (place + s)]);
 #pragma unroll
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedAttnArgs a) 
     o1 *= inv;
     const uint32_t lo = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o0) : __builtin_bit_cast(uint16_t, (_Float16)o0);
     const uint32_t hi = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o1) : __builtin_bit_cast(uint16_t, (_Float16)o1);
-    reinterpret_cast<uint32_t *>(a.out)[((seq.row0 + nth) * heads + head) * 64 + lane] = lo | (hi << 16);
+    reinterpret_cast<uint32_t *>(a.out)[((int64_t)(seq.row0 + nth) * heads + head) * 64 + lane] = lo | (hi << 16);
 }
 
 struct Plan {

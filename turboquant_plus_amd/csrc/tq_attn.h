@@ -221,11 +221,16 @@ __device__ __forceinline__ PagedPass paged_pass(const AttnArgs &a, int group, in
     PagedPass g;
     g.kvh = group - (int)(b * a.pg.r.heads_div.d);
     const tq_pages &p = a.pg.r.p;
-    const int32_t lo = p.cu_new ? scalar_entry(p.cu_new, b) : (int32_t)b, hi = p.cu_new ? scalar_entry(p.cu_new, b + 1) : (int32_t)b + 1;
+    const int32_t len = scalar_entry(p.lens, b);
+    int32_t lo = (int32_t)b, hi = lo + 1;
+    if (p.cu_new) {   // one branch: the three loads are on their way together
+        lo = scalar_entry(p.cu_new, b);
+        hi = scalar_entry(p.cu_new, b + 1);
+    }
     g.row0 = lo;
     g.n = lo >= 0 && hi > lo && hi <= a.pg.r.rows ? hi - lo : 0;
     g.rows = min(g.n, a.pg.max_new) * (int)a.pg.heads_div.d;
-    g.ctx = min(max(scalar_entry(p.lens, b), 0), a.pg.max_context);
+    g.ctx = min(max(len, 0), a.pg.max_context);
     const bool some = head_off < g.rows;
     g.least = some ? paged_limit(a, g, head_off) : 0;
     g.most = some ? paged_limit(a, g, min(head_off + heads, g.rows) - 1) : 0;

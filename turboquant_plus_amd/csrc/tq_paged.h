@@ -17,9 +17,9 @@ struct PagedRows {
 };
 
 struct PagedSeq {
-    int64_t row0;   // its first row in the new tokens' tensors
+    int row0;       // its first row in the new tokens' tensors
     int n;          // its rows; 0 where the tables give rows outside of the tensors
-    int64_t start;  // lens[b]
+    int start;      // lens[b]
 };
 __device__ __forceinline__ PagedSeq paged_seq(const PagedRows &r, int b) {
     PagedSeq q;
@@ -31,13 +31,12 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedRows &r, int b) {
 }
 // whether an append at lens[b] has a place for the sequence's rows
 __device__ __forceinline__ bool paged_room(const PagedRows &r, const PagedSeq &q) {
-    return q.start >= 0 && q.start + q.n <= (int64_t)r.p.max_blocks * TQ_ROWS_PER_BLOCK;
+    return q.start >= 0 && (int64_t)q.start + q.n <= (int64_t)r.p.max_blocks * TQ_ROWS_PER_BLOCK;
 }
-// blocks that hold rows of sequence b
-__device__ __forceinline__ int paged_blocks(const PagedRows &r, int b) {
-    const PagedSeq q = paged_seq(r, b);
+// blocks that hold rows of a sequence
+__device__ __forceinline__ int paged_blocks(const PagedRows &r, const PagedSeq &q) {
     if (q.n == 0 || !paged_room(r, q)) return 0;
-    return (int)((q.start + q.n - 1) / TQ_ROWS_PER_BLOCK - q.start / TQ_ROWS_PER_BLOCK) + 1;
+    return (q.start + q.n - 1) / TQ_ROWS_PER_BLOCK - q.start / TQ_ROWS_PER_BLOCK + 1;
 }
 // One workgroup's look at every sequence: why an append leaves some out.
 __device__ __forceinline__ void paged_report(const PagedRows &r, uint32_t *overrun) {
@@ -52,24 +51,41 @@ __device__ __forceinline__ void paged_report(const PagedRows &r, uint32_t *overr
     }
 }
 
-// Item `item` of the sequences' items laid end to end, count(b) of them to sequence b: its sequence and its number there, the
+// sum over the lanes up to this one
+__device__ __forceinline__ int sum_upto_lane(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // from one, two, four, eight lanes down in a row of sixteen
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // the rows' sums: rows 0 and 2 to 1 and 3, then row 1's to 2 and 3
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+}
+// Item `item` of the sequences' items laid end to end, count(sequence) of them to each: its sequence and its number there, the
 // same in every lane; false behind the last one.  Every wavefront of a workgroup calls it and works it out for itself: 64
 // sequences at a time, a sum over the lanes.
-template <class Count> __device__ __forceinline__ bool paged_item(const PagedRows &r, int item, Count count, int &b, int &nth) {
+template <class Count> __device__ __forceinline__ bool paged_item(const PagedRows &r, int item, Count count, int &b, int &nth, PagedSeq &seq) {
     const int lane = (int)(threadIdx.x & 63);
+    if (!r.p.cu_new) {   // one row each, and no more than one item
+        if (item >= r.p.batch) return false;
+        b = item;
+        nth = 0;
+        seq = PagedSeq{item, 1, scalar_entry(r.p.lens, item)};
+        return count(seq) > 0;
+    }
     for (int b0 = 0; b0 < r.p.batch; b0 += 64) {
-        const int c = b0 + lane < r.p.batch ? count(b0 + lane) : 0;
-        int upto = c;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int below = __shfl_up(upto, o);
-            if (lane >= o) upto += below;
+        PagedSeq q{0, 0, 0};
+        int c = 0;
+        if (b0 + lane < r.p.batch) {
+            q = paged_seq(r, b0 + lane);
+            c = count(q);
         }
+        const int upto = sum_upto_lane(c);
         const unsigned long long behind = __builtin_amdgcn_ballot_w64(upto > item);
         if (behind) {
             const int at = __builtin_ctzll(behind);
             b = b0 + at;
             nth = item - __builtin_amdgcn_readlane(upto - c, at);
+            seq = PagedSeq{__builtin_amdgcn_readlane(q.row0, at), __builtin_amdgcn_readlane(q.n, at), __builtin_amdgcn_readlane(q.start, at)};
             return true;
         }
         item -= __builtin_amdgcn_readlane(upto, 63);

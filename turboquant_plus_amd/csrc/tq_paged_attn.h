@@ -190,9 +190,9 @@ __device__ __forceinline__ PagedBlock paged_block(const PagedAttnArgs &a, int it
         nth = item - b * a.blocks_each;
         some = b < a.r.p.batch;
         if (!some) b = 0;
-    } else some = paged_item(a.r, item, [&](int s) { return (min(paged_seq(a.r, s).n, a.max_new) * a.group + rows - 1) / rows; }, b, nth);
-    if (some) {
         k.seq = paged_seq(a.r, b);
+    } else some = paged_item(a.r, item, [&](const PagedSeq &q) { return (min(q.n, a.max_new) * a.group + rows - 1) / rows; }, b, nth, k.seq);
+    if (some) {
         k.span = paged_span(a, k.seq);
         k.n_rows = min(k.seq.n, a.max_new) * a.group;
         k.r0 = nth * rows;
@@ -218,7 +218,7 @@ __device__ __forceinline__ void load_queries(const PagedAttnArgs &a, const Paged
         const int t = (int)a.group_div.div((uint32_t)r), g = r - t * a.group;
         seen[rb] = row_limit(a, k, r);
         float x[32];
-        const int64_t at = (k.seq.row0 + t) * a.q_token + (int64_t)(head * a.group + g) * a.q_head + 32 * kq;
+        const int64_t at = (int64_t)(k.seq.row0 + t) * a.q_token + (int64_t)(head * a.group + g) * a.q_head + 32 * kq;
         if (k.active) {
             const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + at);
 #pragma unroll
@@ -354,7 +354,7 @@ __device__ __forceinline__ void leave_rows(const PagedAttnArgs &a, const PagedBl
         if (k.span.splits <= 1) {
             write_out(a, x, l[rb] > 0.0f ? a.v_unscale / l[rb] : l[rb] == 0.0f ? 0.0f : l[rb], k.seq.row0 + t, hq, there, lane);
         } else if (there) {
-            const int64_t at = ((k.seq.row0 + t) * (a.r.p.n_kv_heads * a.group) + hq) * a.n_splits + split;
+            const int64_t at = ((int64_t)(k.seq.row0 + t) * (a.r.p.n_kv_heads * a.group) + hq) * a.n_splits + split;
 #pragma unroll
             for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(a.part_o + at * 128 + out_dim(e, kq)) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
             if (kq == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * at) = make_float2(m[rb], l[rb]);

@@ -3278,8 +3278,11 @@ __global__ __launch_bounds__(256) void k_q8_0_unpack(const uint8_t *packed, int8
 // Rows of several sequences, token-major, appended to pages: a workgroup per touched block and side, on the code of the
 // contiguous appends (append_unit_rows, q8_0_append_rows), so the bytes are theirs.  Which sequence and block a workgroup has, it
 // finds by itself from the sequences' lengths in device memory (paged_item), so the grid is only an upper bound.
-// Bound by vector instructions, as the contiguous appends are.
-template <typename TI>
+// Bound by vector instructions, as the contiguous appends are: 16384 new rows of 8 heads, turbo4, fp16: 34 us (contiguous 32; 84 MB, 2.5
+// TB/s).  Single tokens wait for memory three times in turn, for lengths, page and row: 64 x 8 heads, turbo3, 10.3 us (contiguous 6.5).
+// BITS: turbo rows of one width on both sides, 0: any; kernels of their own use less registers and no shared memory (that step 11.6
+// -> 10.3 us, the prompt 34.3 -> 34.0).
+template <typename TI, int BITS>
 __global__ __launch_bounds__(APPEND_THREADS, (std::is_same<TI, __half>::value ? 4 : 3)) void k_append_paged(PagedRows r, const TI *xk, const TI *xv, uint8_t *pk,
                                                                                uint8_t *pv, int64_t k_token, int64_t k_head, int64_t v_token,
                                                                                int64_t v_head, int kb, int vb, int k_wide, int v_wide,
@@ -3290,12 +3293,11 @@ __global__ __launch_bounds__(APPEND_THREADS, (std::is_same<TI, __half>::value ? 
     const uint32_t item = r.heads_div.div(wg), head = wg - item * r.heads_div.d;
     if (overrun && blockIdx.x == 0) paged_report(r, overrun);
     int b, nth;
-    if (!paged_item(r, (int)item, [&](int s) { return paged_blocks(r, s); }, b, nth)) return;
-    const PagedSeq q = paged_seq(r, b);
-    const int64_t bis = q.start / TQ_ROWS_PER_BLOCK + nth, tok0 = bis * TQ_ROWS_PER_BLOCK;
-    const int n_old = (int)(q.start - tok0 < 0 ? 0 : q.start - tok0);
-    const int n_end = (int)(q.start + q.n - tok0 > TQ_ROWS_PER_BLOCK ? TQ_ROWS_PER_BLOCK : q.start + q.n - tok0);
-    const int page = __builtin_amdgcn_readfirstlane(r.p.block_table[b * r.p.table_stride + bis]);
+    PagedSeq q;
+    if (!paged_item(r, (int)item, [&](const PagedSeq &s) { return paged_blocks(r, s); }, b, nth, q)) return;
+    const int bis = q.start / TQ_ROWS_PER_BLOCK + nth, tok0 = bis * TQ_ROWS_PER_BLOCK;
+    const int n_old = max(q.start - tok0, 0), n_end = min(q.start + q.n - tok0, TQ_ROWS_PER_BLOCK);
+    const int page = scalar_entry(r.p.block_table, b * r.p.table_stride + bis);
     if (page < 0 || page >= r.p.n_pages) {
         if (overrun && threadIdx.x == 0 && !is_v && head == 0) atomicOr(overrun, TQ_OVERRUN_NO_PAGE);
         return;
@@ -3303,9 +3305,12 @@ __global__ __launch_bounds__(APPEND_THREADS, (std::is_same<TI, __half>::value ? 
     const int64_t at = (int64_t)page * r.p.n_kv_heads + head;
     const TI *x = is_v ? xv + head * v_head : xk + head * k_head;
     const int64_t step = is_v ? v_token : k_token;
-    x += (q.row0 + (tok0 - q.start)) * step;
+    x += (int64_t)(q.row0 + (tok0 - q.start)) * step;
     auto row = [&](int t) { return x + t * step; };
-    if (!is_v) {
+    if constexpr (BITS != 0) {
+        if (!is_v) append_unit_rows<BITS, TQ_KIND_K, false, TI>(row, pk + at * block_bytes(BITS), n_old, n_end, ka);
+        else append_unit_rows<BITS, TQ_KIND_V, false, TI>(row, pv + at * block_bytes(BITS), n_old, n_end, va);
+    } else if (!is_v) {
         switch (kb) {
         case 2: append_unit_rows<2, TQ_KIND_K, false, TI>(row, pk + at * block_bytes(2), n_old, n_end, ka); break;
         case 3: append_unit_rows<3, TQ_KIND_K, false, TI>(row, pk + at * block_bytes(3), n_old, n_end, ka); break;
@@ -3343,6 +3348,15 @@ __device__ __forceinline__ void load_paged_tile(const PagedLoadSide &a, const ui
     const int n16 = lane & 15, kc = lane >> 4;
     constexpr int XROW = LOAD16_XROW, PIECES = BITS * 64 + 8;
     for (int e = tid; e < (1 << (2 * BITS)); e += 256) lut_s[e] = a.lut[e];
+    // whether any of this wavefront's 16 tokens (below) is wanted: of a single one's tile, three wavefronts only help to stage it
+    const bool wanted = KIND == TQ_KIND_K ? lo < 16 * wave + 16 && hi > 16 * wave
+                                          : __builtin_amdgcn_ballot_w64(lo <= 16 * (n16 >> 2) + 4 * wave + (n16 & 3) && 16 * (n16 >> 2) + 4 * wave + (n16 & 3) < hi) != 0ull;
+    if constexpr (KIND == TQ_KIND_V) {
+        for (int e = tid; e < PIECES - 8; e += 256)
+            reinterpret_cast<uint4 *>(tile_s)[e] = *reinterpret_cast<const uint4 *>(block + (e >> 6) * 2048 + (64 * half + (e & 63)) * 16);
+    }
+    __syncthreads();
+    if (!wanted) return;
     half8_t af[8];
 #pragma unroll
     for (int f = 0; f < 8; ++f) af[f] = __builtin_bit_cast(half8_t, a.afrag[f * 64 + lane]);
@@ -3358,11 +3372,7 @@ __device__ __forceinline__ void load_paged_tile(const PagedLoadSide &a, const ui
     if constexpr (KIND == TQ_KIND_K) {
 #pragma unroll
         for (int j = 0; j < BITS; ++j) cw[j] = *reinterpret_cast<const uint32_t *>(block + j * 2048 + (64 * half + tl) * 16 + kc * 4);
-    } else {
-        for (int e = tid; e < PIECES - 8; e += 256)
-            reinterpret_cast<uint4 *>(tile_s)[e] = *reinterpret_cast<const uint4 *>(block + (e >> 6) * 2048 + (64 * half + (e & 63)) * 16);
     }
-    __syncthreads();
     uint4 xb[4];
     if constexpr (KIND == TQ_KIND_K) {
         uint32_t tail = 0;
@@ -3442,19 +3452,16 @@ __global__ __launch_bounds__(256) void k_load_paged(PagedRows r, PagedLoadSide k
     const unsigned wg = is_v ? blockIdx.x - side : blockIdx.x;
     const uint32_t item = r.heads_div.div(wg), head = wg - item * r.heads_div.d;
     int b, nth;
-    if (!paged_item(r, (int)item >> 1, [&](int s) { return paged_blocks(r, s); }, b, nth)) return;
-    const PagedSeq q = paged_seq(r, b);
-    const int64_t bis = q.start / TQ_ROWS_PER_BLOCK + nth;
-    const int half = (int)(item & 1);
-    const int64_t tok0 = bis * TQ_ROWS_PER_BLOCK + 64 * half;
-    const int lo = (int)(q.start - tok0 < 0 ? 0 : q.start - tok0 > 64 ? 64 : q.start - tok0);
-    const int hi = (int)(q.start + q.n - tok0 > 64 ? 64 : q.start + q.n - tok0);
+    PagedSeq q;
+    if (!paged_item(r, (int)item >> 1, [&](const PagedSeq &s) { return paged_blocks(r, s); }, b, nth, q)) return;
+    const int bis = q.start / TQ_ROWS_PER_BLOCK + nth, half = (int)(item & 1), tok0 = bis * TQ_ROWS_PER_BLOCK + 64 * half;
+    const int lo = min(max(q.start - tok0, 0), 64), hi = min(q.start + q.n - tok0, 64);
     if (lo >= hi) return;
-    const int page = __builtin_amdgcn_readfirstlane(r.p.block_table[b * r.p.table_stride + bis]);
+    const int page = scalar_entry(r.p.block_table, b * r.p.table_stride + bis);
     if (page < 0 || page >= r.p.n_pages) return;
     const int64_t at = (int64_t)page * r.p.n_kv_heads + head, step = (int64_t)r.p.n_kv_heads * 128;
     const PagedLoadSide &a = is_v ? vs : ks;
-    __half *out = a.out + (q.row0 + (tok0 - q.start)) * step + head * 128;
+    __half *out = a.out + (int64_t)(q.row0 + (tok0 - q.start)) * step + head * 128;
 #define TQ_LOAD_PAGED(B)                                                                                                              if (is_v) load_paged_tile<B, TQ_KIND_V>(vs, vs.pages + at * block_bytes(B), half, lo, hi, out, step, lut_s, tile_s, xpose_s);      else load_paged_tile<B, TQ_KIND_K>(ks, ks.pages + at * block_bytes(B), half, lo, hi, out, step, lut_s, tile_s, xpose_s)
     switch (a.bits) {
     case 2: TQ_LOAD_PAGED(2); break;
@@ -4955,10 +4962,19 @@ int tqk_append_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *p
     auto wide = [&](const void *x, int64_t token, int64_t head) {
         return (int)(reinterpret_cast<uintptr_t>(x) % 16 == 0 && token * each % 16 == 0 && head * each % 16 == 0);
     };
-#define TQ_APPEND_PAGED(T)                                                                                                                    k_append_paged<T><<<(unsigned)grid, APPEND_THREADS, 0, s>>>(r, (const T *)k, (const T *)v, (uint8_t *)k_pages, (uint8_t *)v_pages, k_token,                                                                 k_head, v_token, v_head, hk ? hk->bits : 0, hv ? hv->bits : 0,                                                                             wide(k, k_token, k_head), wide(v, v_token, v_head), ka, va, overrun)
-    if (in_dtype == TQ_F16) TQ_APPEND_PAGED(__half);
-    else if (in_dtype == TQ_BF16) TQ_APPEND_PAGED(__bf16);
-    else TQ_APPEND_PAGED(float);
+    const int kb = hk ? hk->bits : 0, vb = hv ? hv->bits : 0;
+#define TQ_APPEND_PAGED(T, B)                                                                                                     \
+    k_append_paged<T, B><<<(unsigned)grid, APPEND_THREADS, 0, s>>>(r, (const T *)k, (const T *)v, (uint8_t *)k_pages, (uint8_t *)v_pages, k_token, \
+                                                                 k_head, v_token, v_head, kb, vb, wide(k, k_token, k_head), wide(v, v_token, v_head), ka, va, overrun)
+#define TQ_APPEND_WIDTHS(T)                                  \
+    if (kb == 2 && vb == 2) TQ_APPEND_PAGED(T, 2);           \
+    else if (kb == 3 && vb == 3) TQ_APPEND_PAGED(T, 3);      \
+    else if (kb == 4 && vb == 4) TQ_APPEND_PAGED(T, 4);      \
+    else TQ_APPEND_PAGED(T, 0)
+    if (in_dtype == TQ_F16) { TQ_APPEND_WIDTHS(__half); }
+    else if (in_dtype == TQ_BF16) { TQ_APPEND_WIDTHS(__bf16); }
+    else { TQ_APPEND_WIDTHS(float); }
+#undef TQ_APPEND_WIDTHS
 #undef TQ_APPEND_PAGED
     return tq_check_launch("append_paged");
 }

@@ -34,47 +34,57 @@ def _handle(codec):
     return None if codec is None else codec.handle.h
 
 
-def _here(name, x, device):
-    if not x.is_cuda or x.get_device() != device:
-        raise ValueError(f"{name} must be on the current device")
+def _refuse_place(device, **tensors):
+    for name, x in tensors.items():
+        if x is not None and x.get_device() != device:     # -1: host memory
+            raise ValueError(f"{name} must be on the current device")
 
+
+# The checks below are most of what a call on a few tokens takes on the host (14 us a call at first, 4 of them the launch), so each asks
+# a tensor once and no name is made before something is wrong.
 
 def _pages(k_codec, v_codec, k_pages, v_pages, block_table, lens, cu_new, device) -> L.TQPages:
     tt = L.torch()
-    for name, x, codec in (("k_pages", k_pages, k_codec), ("v_pages", v_pages, v_codec)):
-        if x.dtype != tt.uint8 or x.dim() != 3 or x.shape[2] != page_bytes(codec) or not x.is_contiguous():
+    k_shape, v_shape = k_pages.shape, v_pages.shape
+    for name, x, shape, codec in (("k_pages", k_pages, k_shape, k_codec), ("v_pages", v_pages, v_shape, v_codec)):
+        if x.dtype is not tt.uint8 or len(shape) != 3 or shape[2] != page_bytes(codec) or not x.is_contiguous():
             raise ValueError(f"{name} must be a contiguous uint8 tensor [pages, KV heads, {page_bytes(codec)}]")
-        _here(name, x, device)
-    if k_pages.shape[:2] != v_pages.shape[:2]:
+    if k_shape[:2] != v_shape[:2]:
         raise ValueError("k_pages and v_pages must have the same pages and KV heads")
-    if block_table.dtype != tt.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype is not tt.int32 or block_table.dim() != 2:
         raise ValueError("block_table must be int32 [batch, blocks], a sequence's entries next to each other")
-    batch = block_table.shape[0]
-    if lens.dtype != tt.int32 or tuple(lens.shape) != (batch,) or not lens.is_contiguous():
+    (batch, blocks), (row, entry) = block_table.shape, block_table.stride()
+    if blocks > 1 and entry != 1:
+        raise ValueError("block_table must be int32 [batch, blocks], a sequence's entries next to each other")
+    if lens.dtype is not tt.int32 or lens.shape != (batch,) or not lens.is_contiguous():
         raise ValueError("lengths must be a contiguous int32 tensor [batch]")
+    cu = None
     if cu_new is not None:
-        if cu_new.dtype != tt.int32 or tuple(cu_new.shape) != (batch + 1,) or not cu_new.is_contiguous():
+        if cu_new.dtype is not tt.int32 or cu_new.shape != (batch + 1,) or not cu_new.is_contiguous():
             raise ValueError("cu_new must be a contiguous int32 tensor [batch + 1]")
-        _here("cu_new", cu_new, device)
-    _here("block_table", block_table, device)
-    _here("lengths", lens, device)
-    return L.TQPages(batch, k_pages.shape[1], k_pages.shape[0], block_table.shape[1],
-                     block_table.stride(0) if batch > 1 else block_table.shape[1], block_table.data_ptr(),
-                     None if cu_new is None else cu_new.data_ptr(), lens.data_ptr())
+        cu = cu_new.data_ptr()
+    if (k_pages.get_device() != device or v_pages.get_device() != device or block_table.get_device() != device or lens.get_device() != device
+            or (cu is not None and cu_new.get_device() != device)):
+        _refuse_place(device, k_pages=k_pages, v_pages=v_pages, cu_new=cu_new, block_table=block_table, lengths=lens)
+    return L.TQPages(batch, k_shape[1], k_shape[0], blocks, row if batch > 1 else blocks, block_table.data_ptr(), cu, lens.data_ptr())
 
 
-def _rows(name, x, heads, device):
-    """Rows [rows, heads, 128] whose values lie next to each other."""
-    if x.dim() != 3 or x.shape[2] != HEAD_DIM or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{name} must be [rows, {'heads' if heads is None else heads}, {HEAD_DIM}], got {tuple(x.shape)}")
-    _here(name, x, device)
-    return x if x.stride(2) == 1 else x.contiguous()
+def _rows(name, x, heads, device, step):
+    """(x, its strides): rows [rows, heads, 128] whose values lie next to each other, and which begin at multiples of 16 bytes (`step`
+    values); a copy where they do not."""
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM or shape[1] != heads:
+        raise ValueError(f"{name} must be [rows, {heads}, {HEAD_DIM}], got {tuple(shape)}")
+    if x.get_device() != device:
+        _refuse_place(device, **{name: x})
+    strides = x.stride()
+    if strides[2] != 1 or strides[0] % step or strides[1] % step or x.data_ptr() % 16:
+        x = x.clone(memory_format=L.torch().contiguous_format)
+        strides = x.stride()
+    return x, strides
 
 
-def _aligned(x, each):
-    """x, or a copy of it whose rows begin at multiples of 16 bytes."""
-    step = 16 // each
-    return x if x.data_ptr() % 16 == 0 and x.stride(0) % step == 0 and x.stride(1) % step == 0 else x.clone(memory_format=L.torch().contiguous_format)
+_APPENDED = {}      # torch dtype -> its code
 
 
 def append_paged(k_codec: TurboCodec | None, v_codec: TurboCodec | None, k, v, k_pages, v_pages, block_table, starts, cu_new=None, *,
@@ -86,17 +96,22 @@ def append_paged(k_codec: TurboCodec | None, v_codec: TurboCodec | None, k, v, k
     `overrun` (a zeroed int32 device tensor with one element) then collects OVERRUN_* bits, see overrun_bits()."""
     tt, device = L.torch(), L._current_device()
     pages = _pages(k_codec, v_codec, k_pages, v_pages, block_table, starts, cu_new, device)
-    k, v = _rows("k", k, pages.n_kv_heads, device), _rows("v", v, pages.n_kv_heads, device)
-    if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
+    dtype, heads = k.dtype, k_pages.shape[1]
+    code = _APPENDED.get(dtype)
+    if code is None:
+        _APPENDED.update({tt.float16: L.TQ_F16, tt.bfloat16: L.TQ_BF16, tt.float32: L.TQ_F32})
+        code = _APPENDED.get(dtype)
+        if code is None:
+            raise TypeError(f"unsupported dtype {dtype}")
+    step = 4 if code == L.TQ_F32 else 8
+    k, ks = _rows("k", k, heads, device, step)
+    v, vs = _rows("v", v, heads, device, step)
+    rows = k.shape[0]
+    if rows != v.shape[0] or v.dtype is not dtype:
         raise ValueError("k and v must have the same rows and dtype")
-    code = L.TQ_BF16 if k.dtype == tt.bfloat16 else L.dtype_code(k)
-    if code == L.TQ_F64:
-        raise TypeError("unsupported dtype torch.float64")
-    each = k.element_size()
-    k, v = _aligned(k, each), _aligned(v, each)
-    L.check(L.lib().tq_append_paged(_handle(k_codec), _handle(v_codec), C.byref(pages), k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0),
-                                    k.stride(1), v.stride(0), v.stride(1), code, k_pages.data_ptr(), v_pages.data_ptr(),
-                                    _overrun_ptr(overrun), L.stream_ptr()))
+    L.check(L.lib().tq_append_paged(_handle(k_codec), _handle(v_codec), C.byref(pages), k.data_ptr(), v.data_ptr(), rows, ks[0], ks[1], vs[0], vs[1],
+                                    code, k_pages.data_ptr(), v_pages.data_ptr(), None if overrun is None else _overrun_ptr(overrun),
+                                    L.stream_ptr()))
     return k_pages, v_pages
 
 
@@ -107,19 +122,21 @@ def load_paged(k_codec: TurboCodec | None, v_codec: TurboCodec | None, k_pages, 
     tensors to write to instead.  Rows behind the last sequence, and rows without a page, are left as they were."""
     tt, device = L.torch(), L._current_device()
     pages = _pages(k_codec, v_codec, k_pages, v_pages, block_table, starts, cu_new, device)
-    if out is not None:
-        rows = out[0].shape[0]
-    elif rows is None:
-        if cu_new is not None:
-            raise ValueError("load_paged needs the number of rows (rows, or out)")
-        rows = pages.batch
-    shape = (rows, pages.n_kv_heads, HEAD_DIM)
     if out is None:
-        out = tuple(tt.empty(shape, dtype=tt.float16, device=k_pages.device) for _ in range(2))
-    for x in out:
-        if x.dtype != tt.float16 or tuple(x.shape) != shape or not x.is_contiguous():
-            raise ValueError(f"outputs must be contiguous fp16 tensors {shape}")
-        _here("out", x, device)
+        if rows is None:
+            if cu_new is not None:
+                raise ValueError("load_paged needs the number of rows (rows, or out)")
+            rows = pages.batch
+        shape = (rows, pages.n_kv_heads, HEAD_DIM)
+        out = k_pages.new_empty(shape, dtype=tt.float16), k_pages.new_empty(shape, dtype=tt.float16)
+    else:
+        rows = out[0].shape[0]
+        shape = (rows, pages.n_kv_heads, HEAD_DIM)
+        for x in out:
+            if x.dtype != tt.float16 or x.shape != shape or not x.is_contiguous():
+                raise ValueError(f"outputs must be contiguous fp16 tensors {shape}")
+            if x.get_device() != device:
+                _refuse_place(device, out=x)
     L.check(L.lib().tq_load_paged(_handle(k_codec), _handle(v_codec), C.byref(pages), k_pages.data_ptr(), v_pages.data_ptr(), rows,
                                   out[0].data_ptr(), out[1].data_ptr(), L.stream_ptr()))
     return out
@@ -156,26 +173,28 @@ class PagedAttention:
         pages = _pages(self.k_codec, self.v_codec, k_pages, v_pages, block_table, lens, cu_new, device)
         if pages.n_kv_heads != self.n_kv_heads:
             raise ValueError(f"pages of {pages.n_kv_heads} KV heads, expected {self.n_kv_heads}")
-        q = _rows("q", q, self.n_q_heads, device)
-        if q.dtype not in (tt.float16, tt.bfloat16):
-            raise TypeError(f"queries must be float16 or bfloat16, not {q.dtype}")
-        q = _aligned(q, 2)
+        dtype = q.dtype
+        if dtype is not tt.float16 and dtype is not tt.bfloat16:
+            raise TypeError(f"queries must be float16 or bfloat16, not {dtype}")
+        q, (q_token, q_head, _) = _rows("q", q, self.n_q_heads, device, 8)
         if out is None:
-            out = tt.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            out = q.new_empty(q.shape)
+        elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor of q's shape and dtype")
-        else:
-            _here("out", out, device)
-        p = L.TQPagedAttnParams(pages, self.n_q_heads, self.causal, self.scale, L.TQ_BF16 if q.dtype == tt.bfloat16 else L.TQ_F16, q.shape[0],
-                                q.stride(0), q.stride(1), 0 if max_context is None else max_context, 0 if max_new is None else max_new)
-        need = L.lib().tq_paged_attn_workspace_bytes(C.byref(p))
+        elif out.get_device() != device:
+            _refuse_place(device, out=out)
+        p = L.TQPagedAttnParams(pages, self.n_q_heads, self.causal, self.scale, L.TQ_BF16 if dtype is tt.bfloat16 else L.TQ_F16, q.shape[0],
+                                q_token, q_head, 0 if max_context is None else max_context, 0 if max_new is None else max_new)
+        lib, at = L.lib(), C.byref(p)
+        need = lib.tq_paged_attn_workspace_bytes(at)
         if need < 0:
             L.check(L.ERR_ARG)
-        if self.workspace is None or self.workspace.numel() < need or self.workspace.get_device() != device:
+        room = -1 if self.workspace is None or self.workspace.get_device() != device else self.workspace.numel()
+        if room < need:
             if self.workspace is not None:
                 self._outgrown.append(self.workspace)     # a captured call may still write to it
             self.workspace = tt.empty(need, dtype=tt.uint8, device=q.device)
-        L.check(L.lib().tq_paged_attention(_handle(self.k_codec), _handle(self.v_codec), C.byref(p), q.data_ptr(), k_pages.data_ptr(),
-                                           v_pages.data_ptr(), out.data_ptr(), self.workspace.data_ptr(), self.workspace.numel(),
-                                           L.stream_ptr()))
+            room = need
+        L.check(lib.tq_paged_attention(_handle(self.k_codec), _handle(self.v_codec), at, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                       out.data_ptr(), self.workspace.data_ptr(), room, L.stream_ptr()))
         return out

@@ -91,37 +91,47 @@ class Rotary:
         some = q if q is not None else k
         if some is None:
             raise ValueError("neither q nor k")
-        dtype, tokens, dim = some.dtype, some.shape[0], some.shape[-1]
-        device = L._current_device()
+        dtype, device = some.dtype, L._current_device()
+        code = _DTYPES.get(dtype)
+        if code is None:
+            _DTYPES.update({tt.float16: L.TQ_F16, tt.float32: L.TQ_F32, tt.bfloat16: L.TQ_BF16})
+            code = _DTYPES.get(dtype)
+        tokens, dim = some.shape[0], some.shape[-1]
         for x in (q, k):
-            if x is not None and (x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != dim or x.dtype != dtype):
+            if x is not None and (len(x.shape) != 3 or x.shape[0] != tokens or x.shape[2] != dim or x.dtype is not dtype):
                 raise ValueError("q and k must be [tokens, heads, head_dim] with the same tokens, head_dim and dtype")
         if out is None:
-            out = tuple(None if x is None else tt.empty(x.shape, dtype=dtype, device=x.device) for x in (q, k))
+            out = None if q is None else q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
         elif len(out) != 2 or any((x is None) != (o is None) or (o is not None and (o.shape != x.shape or o.dtype != dtype))
                                   for x, o in zip((q, k), out)):
             raise ValueError("out must be a pair of tensors of q's and k's shapes and dtype")
-        if positions.dtype not in (tt.int32, tt.int64) or tuple(positions.shape) != (tokens,):
+        index = positions.dtype
+        if (index is not tt.int32 and index is not tt.int64) or positions.shape != (tokens,):
             raise ValueError("positions must be int32 or int64 [tokens]")
         if not positions.is_contiguous():
             positions = positions.contiguous()
-        for x in (q, k, *out, positions, self.turns):
-            if x is not None and (not x.is_cuda or x.get_device() != device):
-                raise ValueError("q, k, positions and the frequencies must be on the current device")
-        for x in (q, k, *out):
-            if x is not None and dim > 1 and x.stride(2) != 1:
+        # (heads, strides and address of q and its output, then of k)
+        sides = []
+        for x, o in ((q, out[0]), (k, out[1])):
+            if x is None:
+                sides.append((0, 0, 0, 0, 0, None, None))
+                continue
+            if x.get_device() != device or o.get_device() != device:
+                raise ValueError(_PLACE)
+            (a, b, c), (d, e, f) = x.stride(), o.stride()
+            if dim > 1 and (c != 1 or f != 1):
                 raise ValueError("a head's values must be next to each other")
-        if dtype not in _DTYPES:
-            _DTYPES.update({tt.float16: L.TQ_F16, tt.float32: L.TQ_F32, tt.bfloat16: L.TQ_BF16})
-            if dtype not in _DTYPES:
-                raise TypeError(f"unsupported dtype {dtype}")
-        strides = lambda x: (x.stride(0), x.stride(1)) if x is not None else (0, 0)
-        p = L.TQRotaryParams(tokens, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], dim, self.rotary_dim, self.interleaved,
-                             inverse, _DTYPES[dtype], positions.dtype == tt.int64, self.magnitude, *strides(q), *strides(k),
-                             *strides(out[0]), *strides(out[1]))
-        L.check(L.lib().tq_rotary(C.byref(p), L.ptr(q), L.ptr(out[0]), L.ptr(k), L.ptr(out[1]), L.ptr(positions), L.ptr(self.turns),
-                                  L.stream_ptr()))
+            sides.append((x.shape[1], a, b, d, e, x.data_ptr(), o.data_ptr()))
+        if positions.get_device() != device or self.turns.get_device() != device:
+            raise ValueError(_PLACE)
+        if code is None:
+            raise TypeError(f"unsupported dtype {dtype}")
+        (hq, qa, qb, oa, ob, q_at, oq_at), (hk, ka, kb, pa, pb, k_at, ok_at) = sides
+        p = L.TQRotaryParams(tokens, hq, hk, dim, self.rotary_dim, self.interleaved, inverse, code, index is tt.int64, self.magnitude, qa, qb,
+                             ka, kb, oa, ob, pa, pb)
+        L.check(L.lib().tq_rotary(C.byref(p), q_at, oq_at, k_at, ok_at, positions.data_ptr(), self.turns.data_ptr(), L.stream_ptr()))
         return out
 
 
-_DTYPES = {}
+_DTYPES = {}      # torch dtype -> its code
+_PLACE = "q, k, positions and the frequencies must be on the current device"
