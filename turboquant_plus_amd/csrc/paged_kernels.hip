@@ -77,6 +77,11 @@ struct Formats {
     int kb, vb;    // code widths, 8 for 8-bit rows
     bool share;    // one codebook
 };
+// The decode kernels: four rows per pass, or eight, and as many wavefronts as the chip holds at once, each with two tiles at least (16 x 8
+// groups at 32K, turbo3, us: 93; twice as many wavefronts 102, four times 125; 32 ragged sequences 117, 126, 147).  Workgroups are
+// shared among groups, cut to make one for every CU, and run by k_decode_turbo with its larger tables as in a step over contiguous
+// caches.  A workgroup's share of the tiles follows from max_context: sequences that are shorter leave workgroups idle, which end
+// at once, and none has more to do than another.
 bool plan_few(const tq_paged_attn_params *p, const Formats &f, int64_t most, Plan &pl) {
     const bool turbo_k = f.kb != 8, turbo_v = f.vb != 8;
     pl.hg = most > 4 ? 2 : 1;
@@ -121,15 +126,21 @@ bool make_plan(const tq_paged_attn_params *p, const Formats &f, Plan &pl) {
     pl.max_new = (int)max_new;
     const int64_t most = max_new * group, space = (int64_t)p->pages.max_blocks * TQ_ROWS_PER_BLOCK;
     pl.max_context = (int)(p->max_context > 0 ? std::min<int64_t>(p->max_context, space) : space);
+    // Up to two passes of eight rows the decode kernels are ahead, whose loads are a row to a lane (16 ragged sequences of up to 8000
+    // positions, 8 KV heads, turbo3, us: 16 rows 47; 24 rows three passes 68, ROWS_32 59, CHUNK_128 107).  Then a wavefront
+    // that decodes for itself (40 rows ROWS_48 80, CHUNK_128 115), then shared operands (64 rows CHUNK_64 96, CHUNK_128 113; 128 rows
+    // CHUNK_64 162, CHUNK_128 125; 448 rows over 1500 positions, 64 heads, CHUNK_128 81, CHUNK_256 75; 800 rows over 32K 279, 213;
+    // 8192 rows 1414, 1290).
     pl.few = most <= 16;
     if (pl.few) return plan_few(p, f, most, pl);
-    pl.kind = most <= 32 ? ROWS_32 : most <= 48 ? ROWS_48 : most < 1024 ? CHUNK_128 : CHUNK_256;
+    pl.kind = most <= 32 ? ROWS_32 : most <= 48 ? ROWS_48 : most <= 64 ? CHUNK_64 : most < 256 ? CHUNK_128 : CHUNK_256;
     const int64_t tile = rows_of(pl.kind);
     pl.items = std::min(p->pages.batch * ceil_div(most, tile), rows * group / tile + p->pages.batch);
     const int64_t tiles = std::max<int64_t>(1, ceil_div(pl.max_context, 64)), blocks = pl.items * p->pages.n_kv_heads;
-    // wavefronts (chunks: workgroups) that fill the chip, and the least that one is given
+    // wavefronts (chunks: workgroups) that the chip holds at once, and the tiles that one is given at least.  More rounds of smaller parts
+    // even out ragged batches but pay for it in partial results (6 prompts of up to 2501 tokens 321 us, 626 with four times the parts).
     const int w = pl.kind == ROWS_32 || pl.kind == ROWS_48 ? ROWS_WAVES : 1;   // wavefronts that can share a row block
-    const int64_t want = pl.kind == ROWS_32 ? 2048 : pl.kind == ROWS_48 ? 1024 : pl.kind == CHUNK_128 ? 512 : 256, least = w > 1 ? 2 : 8;
+    const int64_t want = pl.kind == ROWS_32 ? 2048 : pl.kind == ROWS_48 ? 1024 : pl.kind == CHUNK_256 ? 256 : 512, least = w > 1 ? 2 : 8;
     pl.kw = 1;
     while (pl.kw < w && blocks * pl.kw < want && tiles >= 2 * pl.kw) pl.kw *= 2;
     const int64_t splits = std::max<int64_t>(1, std::min(ceil_div(want, blocks * pl.kw), tiles / (least * pl.kw)));

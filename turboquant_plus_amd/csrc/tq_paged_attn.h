@@ -1,20 +1,26 @@
-// Attention of new tokens over a paged cache of packed rows: k_paged_attn and k_paged_merge.
+// Attention of several new tokens over a paged cache of packed rows (tq_paged_attention): k_paged_rows for 17 to 48 rows of a KV
+// head (a row: one new token under one query head), k_paged_chunk for more; fewer run on k_decode_attn and k_decode_turbo.
 //
-// A wavefront takes 16 RB rows (a row: one new token under one query head of a KV head) and walks tiles of 64 positions; it
-// needs nobody else until its end.  Codes become fp16 operands of 16x16x32 matrix instructions in its own registers, through
-// decode tables in LDS, and each operand serves the RB row blocks: what a tile costs to decode is paid once per 16 RB rows.
+// Both walk tiles of 64 positions.  Codes become fp16 operands of 16x16x32 matrix instructions through decode tables in LDS, and
+// each operand serves several blocks of 16 rows: what a tile costs to decode is paid once for all of them.
 //   S^T = K Q^T.  A = K: lane (m = lane % 16, kq = lane / 16) holds dims 32 kq .. 32 kq + 31 of a token, which are BITS dwords of its
 //     row (one pair group), 8 of them per step; B = Q likewise, so Q is loaded, rotated and scaled in the layout in which it is
 //     used.  Row m of unit u is token 16 (m / 4) + 4 u + m % 4 of the tile: the result then gives lane (n, kq) the logits of
 //     row n for the tokens 16 kq + 4 u + i.
-//   softmax: running maximum and sum per lane and row block in 32 bits; the maximum goes over the four lanes of a row.
+//   softmax: running maximum and sum per lane and row block in 32 bits; the maximum goes over the four lanes of a row.  A token's norm of
+//     K multiplies the logits in 32 bits (as fp16 operands they would double the error of the result).
 //   O^T = V^T P^T.  B = P: the lane's own 16 weights, rounded to fp16 with the tokens' norms in them (|error| <= 2^-11 of a weight, of
 //     either sign, so a sum of them is as good as its rounding to 16 bits); A = V: rows are dims, lane (m, kq) takes the pair group kq =
 //     tokens 16 kq .. 16 kq + 15 of dims m and 64 + m of a 16-row block.  No exchange between lanes anywhere in the loop but the
 //     maximum.
+// A query's rounding to fp16 is the largest error of a result (5e-4 of its size over 4000 to 32K positions).
 // The result of a lane is 32 dims of a row, and the transposed rotation of V is a butterfly of five stages in registers and two
-// across lanes.  `kw` wavefronts of a workgroup share the positions of one row block and join through LDS at the end;
-// n_splits workgroups share them where rows are few, through partial results in memory (32 bits) and k_paged_merge.
+// across lanes.  Where rows are few, n_splits workgroups share the positions and join through partial results in memory (32
+// bits) and k_paged_merge.
+// One MI355X.  17 to 48 rows are bound by the decoding: 16 ragged sequences of up to 8000 positions, 8 KV heads, turbo3: 24 rows 59 us
+// (k_paged_chunk 107), 40 rows 80 us (115).  Many rows are bound by the matrix instructions with the softmax between them: 2048
+// tokens x 32 heads at the end of 32K positions 1.26 ms, 845 TFLOP/s where a product of 8192^3 fp16 matrices reaches 1159 (vector unit
+// 55 %, matrix unit 35 %, LDS 35 % busy before two tiles of logits were in flight).
 #pragma once
 #include <type_traits>
 
@@ -30,9 +36,9 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 constexpr float RSQRT128 = 0.08838834764831845f;
 
-// How rows are dealt out, by a sequence's most: 32 or 48 to a wavefront that decodes for itself, 128 or 256 to a workgroup
-enum PagedKind { ROWS_32, ROWS_48, CHUNK_128, CHUNK_256 };
-__host__ __device__ constexpr int rows_of(PagedKind k) { return k == ROWS_32 ? 32 : k == ROWS_48 ? 48 : k == CHUNK_128 ? 128 : 256; }
+// How rows are dealt out, by a sequence's most: 32 or 48 to a wavefront that decodes for itself, 64, 128 or 256 to a workgroup
+enum PagedKind { ROWS_32, ROWS_48, CHUNK_64, CHUNK_128, CHUNK_256 };
+__host__ __device__ constexpr int rows_of(PagedKind k) { return k == ROWS_32 ? 32 : k == ROWS_48 ? 48 : k == CHUNK_64 ? 64 : k == CHUNK_128 ? 128 : 256; }
 
 struct PagedAttnArgs {
     PagedRows r;
@@ -677,9 +683,11 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, RB == 2 ? 2 : 1) void k_paged_rows
 }
 
 // ---- many rows: a workgroup decodes a tile once for all of its wavefronts ------------------------------------
-// 32 rows per wavefront, 32 W per workgroup.  Every tile's operands are decoded by the wavefronts in turns of a 16-token unit of K or
-// a 16-dim block of V and lie in LDS as the matrix instructions take them (a lane's 16 bytes next to its neighbour's), a tile ahead
-// of their use, behind one barrier per tile.
+// 16 RB rows per wavefront (RB 1: 64 rows, else 128 or 256 per workgroup).  Every tile's operands are decoded by the wavefronts in
+// turns of a 16-token unit of K or a 16-dim block of V and lie in LDS as the matrix instructions take them (a lane's 16 bytes next
+// to its neighbour's), ahead of their use, behind one barrier per tile: K's two tiles and V's one, so that the next tile's
+// logits are multiplied while this one's weights are worked out (chunk of 2048 at 32K: 3.07 -> 1.33 ms with the shared decoding,
+// wider loads and this order).
 // copies of a decode table: a workgroup looks each pair up once, and two of its size share a CU's LDS
 __host__ __device__ constexpr int chunk_copies(int bits) { return bits == 4 ? 4 : 16; }
 template <int KB, int VB, int W, int RB>

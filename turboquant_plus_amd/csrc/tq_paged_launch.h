@@ -17,6 +17,7 @@ template <int KB, int VB> int launch_kind(const PagedAttnArgs &a, PagedKind kind
     switch (kind) {
     case ROWS_32: launch_rows<KB, VB, 2>(a, grid, s); break;
     case ROWS_48: launch_rows<KB, VB, 3>(a, grid, s); break;
+    case CHUNK_64: k_paged_chunk<KB, VB, 4, 1><<<grid, 256, 0, s>>>(a); break;
     case CHUNK_128: k_paged_chunk<KB, VB, 4, 2><<<grid, 256, 0, s>>>(a); break;
     default: k_paged_chunk<KB, VB, 8, 2><<<grid, 512, 0, s>>>(a); break;
     }
