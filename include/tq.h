@@ -453,7 +453,7 @@ int tq_rotary(const tq_rotary_params *p, const void *q, void *q_out, const void 
  * 0 .. n_pages - 1 are neither read nor written.  No counterpart in the reference, whose cache is rebuilt whole
  * (kv_cache.py:41-66). */
 typedef struct tq_pages {
-    int32_t batch, n_kv_heads;
+    int32_t batch, n_kv_heads;  /* 65536 heads at most, 2^31 - 1 of all sequences      */
     int32_t n_pages;
     int32_t max_blocks;         /* entries of a row of block_table, at most 2^24 - 1  */
     int64_t table_stride;       /* from one sequence's row to the next                 */
@@ -482,7 +482,7 @@ int tq_load_paged(const tq_handle *hk, const tq_handle *hv, const tq_pages *page
 
 /* Attention of new tokens over a paged cache: for row t of the n of sequence b, which holds c = lens[b] tokens,
  *     out = softmax(scale q K^T) V  over the positions before c - n + t + 1 (causal) or before c;
- * a row that sees nothing is 0.  One row (a decode step), a few (drafted tokens), chunks and whole prompts; queries over another
+ * a row that sees nothing is 0; positions whose entry is no page are not seen.  One row (a decode step), a few (drafted tokens), chunks and whole prompts; queries over another
  * sequence's states with causal = 0. */
 typedef struct tq_paged_attn_params {
     tq_pages pages;
@@ -498,7 +498,7 @@ typedef struct tq_paged_attn_params {
 } tq_paged_attn_params;
 /* Bytes of workspace for these parameters (16-byte aligned; it may hold anything; calls that share one must not overlap in time). */
 int64_t tq_paged_attn_workspace_bytes(const tq_paged_attn_params *p);
-/* q, out and pages 16-byte aligned; hk / hv NULL: q8_0-style rows on that side.  Rows behind the last sequence are left as they were. */
+/* q, out and pages 16-byte aligned, out apart from q; hk / hv NULL: q8_0-style rows on that side.  Rows behind the last sequence are left as they were. */
 int tq_paged_attention(const tq_handle *hk, const tq_handle *hv, const tq_paged_attn_params *p, const void *q, const void *k_pages,
                        const void *v_pages, void *out, void *workspace, int64_t workspace_bytes, void *stream);
 

@@ -21,6 +21,7 @@ def attn(page_kw=None, **kw):
 
 BAD_PAGES = [(dict(batch=-1), L.ERR_ARG, "negative"), (dict(n_kv_heads=0), L.ERR_ARG, "negative"), (dict(n_pages=-1), L.ERR_ARG, "negative"),
              (dict(max_blocks=-1), L.ERR_ARG, "negative"), (dict(n_kv_heads=70000), L.ERR_UNSUPPORTED, "65536"),
+             (dict(batch=1 << 20, n_kv_heads=4096), L.ERR_UNSUPPORTED, "of all sequences"),
              (dict(max_blocks=1 << 24, table_stride=1 << 24), L.ERR_UNSUPPORTED, "32 bits"), (dict(table_stride=3), L.ERR_ARG, "table_stride"),
              (dict(block_table=None), L.ERR_ARG, "null"), (dict(lens=None), L.ERR_ARG, "null"), (dict(lens=4098), L.ERR_ALIGN, "aligned"),
              (dict(batch=20, cu_new=None), L.ERR_ARG, "10 rows for 20")]

@@ -210,7 +210,8 @@ int attend_few(const tq_handle *hk, const tq_handle *hv, const tq_paged_attn_par
 int check_pages(const tq_pages *p, int64_t rows, const char *who) {
     REQUIRE(p, TQ_ERR_ARG, "%s: null pages", who);
     REQUIRE(p->batch >= 0 && p->n_kv_heads >= 1 && p->n_pages >= 0 && p->max_blocks >= 0 && rows >= 0, TQ_ERR_ARG, "%s: negative size", who);
-    REQUIRE(p->n_kv_heads <= 65536, TQ_ERR_UNSUPPORTED, "%s: over 65536 KV heads", who);
+    REQUIRE(p->n_kv_heads <= 65536 && (int64_t)p->batch * p->n_kv_heads <= 0x7FFFFFFF, TQ_ERR_UNSUPPORTED,
+            "%s: over 65536 KV heads, or over 2^31 - 1 of all sequences", who);
     REQUIRE(p->max_blocks < (1 << 24) && rows <= 0x7FFFFFFF, TQ_ERR_UNSUPPORTED, "%s: positions and rows have to fit 32 bits", who);
     REQUIRE(p->table_stride >= p->max_blocks || p->batch <= 1, TQ_ERR_ARG, "%s: table_stride %lld is under max_blocks %d", who,
             (long long)p->table_stride, p->max_blocks);

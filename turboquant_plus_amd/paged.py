@@ -165,7 +165,7 @@ class PagedAttention:
         """q [rows, query heads, 128], float16 or bfloat16, original domain -> out of the same shape and dtype, contiguous.
         lens (int32 [batch]): tokens that each sequence's pages hold, the new ones among them; row t of a sequence's n sees the
         positions before lens[b] - n + t + 1 (all lens[b] of them with causal=False), and a row that sees nothing is 0.
-        Rows behind the last sequence are left as they were (`out`: a contiguous tensor to write to).
+        Rows behind the last sequence are left as they were (`out`: a contiguous tensor to write to, apart from q's memory).
         max_context, max_new: no sequence holds more tokens, or has more new ones.  They size the launch: without them the table's
         width and the number of rows do, and a call on short sequences takes longer.  Of a sequence that exceeds them the
         tokens behind max_context are not seen and the rows from max_new on are left as they were."""
