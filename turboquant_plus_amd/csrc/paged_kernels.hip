@@ -316,7 +316,11 @@ int tq_paged_attention(const tq_handle *hk, const tq_handle *hv, const tq_paged_
     a.k = (const uint8_t *)k_pages; a.v = (const uint8_t *)v_pages;
     a.scale = p->scale * 1.4426950408889634f;
     a.v_unscale = 1.0f;
-    if (hk) { a.klut = hk->scaled_lut; a.ks1 = hk->s1_32; a.ks2 = hk->s2_32; a.scale /= hk->value_scale; }
+    if (hk) {
+        a.klut = hk->scaled_lut;
+        a.scale /= hk->value_scale;
+        for (int i = 0; i < 4; ++i) { a.ks1neg[i] = hk->s1neg_host[i]; a.ks2neg[i] = hk->s2neg_host[i]; }
+    }
     if (hv) { a.vlut = hv->scaled_lut; a.vs1 = hv->s1_32; a.vs2 = hv->s2_32; a.v_unscale = 1.0f / hv->value_scale; }
     a.n_splits = pl.n_splits; a.split_tiles = pl.split_tiles; a.kw = pl.kw;
     a.part_o = (float *)workspace;

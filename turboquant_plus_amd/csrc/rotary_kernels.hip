@@ -3,7 +3,8 @@
 // k_rotary: pair (u, w) of a head -> (u cos a - w sin a, w cos a + u sin a), a = position * frequency.  A workgroup takes a few
 //   tokens with all their heads: it works out the cosines and sines of those tokens once (64-bit turns, reduced to a fraction of
 //   one, so that far positions lose nothing), keeps them in LDS and streams the heads past them, 16 bytes of each half of a
-//   pair at a time.
+//   pair at a time.  Bound by memory: 32768 tokens of 32 + 8 heads of 128, fp16, 671 MB in 123.6 us (5.4 TB/s, 128 in a loop of its own);
+//   value by value, where rows do not begin at 16 bytes, 255 us (interleaved 235).
 #include "tq_check.h"
 #include "tq_layout.h"
 

@@ -33,6 +33,7 @@ using namespace tqd;
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr float RSQRT128 = 0.08838834764831845f;
 
@@ -51,7 +52,8 @@ struct PagedAttnArgs {
     FastDiv group_div, heads_div;
     const uint8_t *k, *v;
     const uint32_t *klut, *vlut; // pair tables of value_scale times the codebook
-    const float *ks1, *ks2, *vs1, *vs2;
+    uint32_t ks1neg[4], ks2neg[4];   // negative signs of K's rotation, 32 dims to a word
+    const float *vs1, *vs2;
     float scale;                 // logits' scale * log2(e) / value_scale of K
     float v_unscale;             // 1 / value_scale of V
     int share;                   // K's table is V's
@@ -201,7 +203,8 @@ __device__ __forceinline__ PagedBlock paged_block(const PagedAttnArgs &a, int it
     if (some) {
         k.span = paged_span(a, k.seq);
         k.n_rows = min(k.seq.n, a.max_new) * a.group;
-        k.r0 = nth * rows;
+        // the last block first, which sees the most: short ones are left for the launch's end (8000 new tokens x 32 heads: 865 -> 727 us)
+        k.r0 = (a.causal ? (k.n_rows + rows - 1) / rows - 1 - nth : nth) * rows;
         k.active = k.r0 < k.n_rows && (split < k.span.splits || split == 0);
     }
     return k;
@@ -214,44 +217,75 @@ __device__ __forceinline__ int row_limit(const PagedAttnArgs &a, const PagedBloc
 
 // Queries of RB blocks from row `first` on: 32 values of row n16 of each block, rotated as K's rows are, as fp16 of their size up to
 // a power of two, which joins the logits' scale.  Rows past the last one repeat it.
+// The rotation goes through the matrix cores, whose products with +-1 are exact for either type.  Dim 32 kq + 8 ks + j in and dim
+// 32 kq' + 8 c + 4 h + i out: H's sign is that of (kq' & kq), (c & ks) and (4 h + i) & j together, so two +-1 operands (h) serve the four
+// steps ks, and the sums over ks are a butterfly of four: a quarter of the vector instructions of one of 128 values (40 rows of 16 ragged
+// sequences 84 -> 79 us, 256 x 64 new tokens over themselves 188 -> 162 with the second tile's K requested beside the first's).
 template <int KB, int RB>
 __device__ __forceinline__ void load_queries(const PagedAttnArgs &a, const PagedBlock &k, int first, int head, int lane, half8_t (&qf)[RB][4],
                                              float (&scale)[RB], int (&seen)[RB]) {
     const int n16 = lane & 15, kq = lane >> 4;
+    uint4 w[RB][4];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const int r = min(first + 16 * rb + n16, max(k.n_rows - 1, 0));
         const int t = (int)a.group_div.div((uint32_t)r), g = r - t * a.group;
         seen[rb] = row_limit(a, k, r);
-        float x[32];
         const int64_t at = (int64_t)(k.seq.row0 + t) * a.q_token + (int64_t)(head * a.group + g) * a.q_head + 32 * kq;
-        if (k.active) {
-            const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + at);
+        const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (k.active ? at : 0));
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint4 u = p[c];
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        for (int c = 0; c < 4; ++c) w[rb][c] = p[c];
+    }
+    auto of_quarter = [&](const uint32_t (&x)[4]) { return kq < 2 ? (kq == 0 ? x[0] : x[1]) : (kq == 2 ? x[2] : x[3]); };
+    const uint32_t neg1 = KB != 8 ? of_quarter(a.ks1neg) : 0u, neg2 = KB != 8 ? of_quarter(a.ks2neg) : 0u;
+    uint4 f[2];
+    if constexpr (KB != 8) {
+        const uint32_t one = a.bf16 ? 0x3F803F80u : 0x3C003C00u;
+        const uint32_t d0 = one ^ (__builtin_popcount((n16 >> 2) & kq) & 1 ? 0x80008000u : 0u) ^ (n16 & 1 ? 0x80000000u : 0u);
+        const uint32_t d1 = d0 ^ (n16 & 2 ? 0x80008000u : 0u);
+        f[0] = make_uint4(d0, d1, d0, d1);
+        f[1] = make_uint4(d0, d1, d0 ^ 0x80008000u, d1 ^ 0x80008000u);
+    }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[8 * c + 2 * j] = a.bf16 ? __uint_as_float(w[j] << 16) : half_of(w[j], 0);
-                    x[8 * c + 2 * j + 1] = a.bf16 ? __uint_as_float(w[j] & 0xFFFF0000u) : half_of(w[j], 1);
+    for (int rb = 0; rb < RB; ++rb) {
+        float x[32];
+        if constexpr (KB != 8) {
+            float4_t z[4][2];
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                auto flipped = [&](uint32_t v, int j) {   // the signs of dims 8 ks + 2 j and the next
+                    const int e = 8 * ks + 2 * j;
+                    return v ^ (((neg1 >> e) & 1u) << 15) ^ (((neg1 >> (e + 1)) & 1u) << 31);
+                };
+                const uint4 v = make_uint4(flipped(w[rb][ks].x, 0), flipped(w[rb][ks].y, 1), flipped(w[rb][ks].z, 2), flipped(w[rb][ks].w, 3));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4_t none = {0.f, 0.f, 0.f, 0.f};
+                    if (a.bf16) z[ks][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f[h]), __builtin_bit_cast(bf16x8_t, v), none, 0, 0, 0);
+                    else z[ks][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, f[h]), __builtin_bit_cast(half8_t, v), none, 0, 0, 0);
                 }
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float s01 = z[0][h][i] + z[1][h][i], d01 = z[0][h][i] - z[1][h][i], s23 = z[2][h][i] + z[3][h][i], d23 = z[2][h][i] - z[3][h][i];
+                    x[4 * h + i] = s01 + s23;
+                    x[8 + 4 * h + i] = d01 + d23;
+                    x[16 + 4 * h + i] = s01 - s23;
+                    x[24 + 4 * h + i] = d01 - d23;
+                }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(__float_as_uint(x[e]) ^ (((neg2 >> e) & 1u) << 31));
         } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = 0.0f;
-        }
-        if constexpr (KB != 8) {
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t u[4] = {w[rb][c].x, w[rb][c].y, w[rb][c].z, w[rb][c].w};
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                const float4 s = *reinterpret_cast<const float4 *>(a.ks1 + 32 * kq + e);
-                x[e] *= s.x; x[e + 1] *= s.y; x[e + 2] *= s.z; x[e + 3] *= s.w;
-            }
-            butterfly32x4(x, lane);
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                const float4 s = *reinterpret_cast<const float4 *>(a.ks2 + 32 * kq + e);
-                x[e] *= s.x * RSQRT128; x[e + 1] *= s.y * RSQRT128; x[e + 2] *= s.z * RSQRT128; x[e + 3] *= s.w * RSQRT128;
+                for (int j = 0; j < 4; ++j) {
+                    x[8 * c + 2 * j] = a.bf16 ? __uint_as_float(u[j] << 16) : half_of(u[j], 0);
+                    x[8 * c + 2 * j + 1] = a.bf16 ? __uint_as_float(u[j] & 0xFFFF0000u) : half_of(u[j], 1);
+                }
             }
         }
         float most = 0.0f;
@@ -260,7 +294,7 @@ __device__ __forceinline__ void load_queries(const PagedAttnArgs &a, const Paged
         most = over_row_max(most);
         int ex = most > 0.0f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
         ex = min(max(ex, -100), 120);
-        scale[rb] = __builtin_amdgcn_ldexpf(a.scale, ex);
+        scale[rb] = __builtin_amdgcn_ldexpf(KB != 8 ? a.scale * RSQRT128 : a.scale, ex);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -722,7 +756,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_chunk(PagedAttnArgs a) {
     const int unit = wave & 3, k_token = 16 * (n16 >> 2) + 4 * unit + (n16 & 3), v_row = 16 * unit + n16;
     uint32_t kw[KB == 8 ? 8 : KB], vw[VB == 8 ? 8 : VB], vsc[VB == 8 ? 16 : 1];
     uint16_t kn = 0, vn = 0;
-    auto request_k = [&](int tile, int page) __attribute__((always_inline)) {
+    auto request_k = [&](int tile, int page, auto &kw, uint16_t &kn) __attribute__((always_inline)) {
         const uint8_t *kb = a.k + ((int64_t)(is_page(page) ? page : 0) * a.r.p.n_kv_heads + head) * KBLOCK;
         const int base = 64 * (min(tile, t_end - 1) & 1);
         if (does_k) {
@@ -821,13 +855,16 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_chunk(PagedAttnArgs a) {
         }
     };
 
+    uint32_t kw1[KB == 8 ? 8 : KB];    // the second tile's K, requested with the first
+    uint16_t kn1 = 0;
     int page = 0, page1 = 0, page2 = 0;    // of this tile and the next two
     if (t_begin < t_end) {
         page = page_of(t_begin);
         page1 = page_of(t_begin + 1);
         page2 = page_of(t_begin + 2);
-        request_k(t_begin, page);
+        request_k(t_begin, page, kw, kn);
         request_v(t_begin, page);
+        request_k(t_begin + 1, page1, kw1, kn1);
     }
     if constexpr (KB != 8) build_pair_table<KB, KC>(lut_s, a.klut, tid, 64 * W);
     if constexpr (VB != 8)
@@ -850,10 +887,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_chunk(PagedAttnArgs a) {
     if (t_begin < t_end) {
         decode_k(t_begin & 1);
         decode_v(t_begin & 1);
-        request_k(t_begin + 1, page1);
         request_v(t_begin + 1, page1);
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(kw) / sizeof(kw[0])); ++j) kw[j] = kw1[j];
+        kn = kn1;
         decode_k((t_begin + 1) & 1);
-        request_k(t_begin + 2, page2);
+        request_k(t_begin + 2, page2, kw, kn);
     }
     __syncthreads();
 
@@ -929,7 +968,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_paged_chunk(PagedAttnArgs a) {
         page1 = page2;
         page2 = page_of(tile + 3);
         request_v(tile + 2, page1);
-        request_k(tile + 3, page2);
+        request_k(tile + 3, page2, kw, kn);
         __syncthreads();
     };
     float4_t s[RB][4];     // this tile's logits, with norms and masks
