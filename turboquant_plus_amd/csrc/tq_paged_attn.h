@@ -18,8 +18,8 @@
 // across lanes.  Where rows are few, n_splits workgroups share the positions and join through partial results in memory (32
 // bits) and k_paged_merge.
 // One MI355X.  17 to 48 rows are bound by the decoding: 16 ragged sequences of up to 8000 positions, 8 KV heads, turbo3: 24 rows 59 us
-// (k_paged_chunk 107), 40 rows 80 us (115).  Many rows are bound by the matrix instructions with the softmax between them: 2048
-// tokens x 32 heads at the end of 32K positions 1.26 ms, 845 TFLOP/s where a product of 8192^3 fp16 matrices reaches 1159 (vector unit
+// (k_paged_chunk 107), 40 rows 75 us (115).  Many rows are bound by the matrix instructions with the softmax between them: 2048
+// tokens x 32 heads at the end of 32K positions 1.28 ms, 834 TFLOP/s where a product of 8192^3 fp16 matrices reaches 1159 (vector unit
 // 55 %, matrix unit 35 %, LDS 35 % busy before two tiles of logits were in flight).
 #pragma once
 #include <type_traits>
@@ -205,7 +205,7 @@ __device__ __forceinline__ PagedBlock paged_block(const PagedAttnArgs &a, int it
         k.n_rows = min(k.seq.n, a.max_new) * a.group;
         // the last block first, which sees the most: short ones are left for the launch's end (8000 new tokens x 32 heads: 865 -> 727 us)
         k.r0 = (a.causal ? (k.n_rows + rows - 1) / rows - 1 - nth : nth) * rows;
-        k.active = k.r0 < k.n_rows && (split < k.span.splits || split == 0);
+        k.active = k.r0 >= 0 && k.r0 < k.n_rows && (split < k.span.splits || split == 0);
     }
     return k;
 }
