@@ -307,6 +307,49 @@ def test_what_lies_in_masked_places_does_not_matter(kf, vf, new):
         assert not tt.isfinite(got[new - 1]).any()
 
 
+@pytest.mark.parametrize("kf,vf", [("turbo4", "turbo4"), ("q8_0", "turbo3"), ("turbo2", "q8_0")])
+@pytest.mark.parametrize("new", [1, 3, 7, 12, 16, 40, 80])
+def test_a_block_without_a_page_is_not_seen(kf, vf, new):
+    """In the middle of a context: the result is that of the other blocks (4 to 320 rows)."""
+    lay, c = layer(kf, vf), 3000
+    kp, vp, table = filled(lay, (c,), 1, 35)
+    gen = tt.Generator("cuda").manual_seed(36)
+    q = tt.randn((new, 4, D), generator=gen, device="cuda").half()
+    rest = tt.cat([table[:, :3], table[:, 4:9], table[:, 10:]], 1).contiguous()
+    want, tol = attend64(lay, q, kp, vp, rest, (c - 256,), (new,), False)
+    for none in (-1, kp.shape[0], 2 ** 31 - 1, -2 ** 31):
+        holes = table.clone()
+        holes[0, 3] = holes[0, 9] = none
+        check(lay.paged_attention(4, 1, causal=False)(q, kp, vp, holes, ints([c]), cumulative([new])), want, tol)
+    assert (lay.paged_attention(4, 1)(q, kp, vp, table * 0 - 1, ints([c]), cumulative([new])) == 0).all()
+
+
+@pytest.mark.parametrize("kf,vf", [("turbo4", "turbo4"), ("turbo3", "turbo4"), ("q8_0", "turbo2"), ("turbo2", "q8_0")])
+@pytest.mark.parametrize("hq,new", [(32, 1), (64, 1), (32, 2), (32, 9)])
+def test_masked_places_of_long_batches(kf, vf, hq, new):
+    """The same where workgroups hold several tiles, with 4-bit tables of a copy per lane among them; entries behind the context are no pages."""
+    lay, hkv = layer(kf, vf), 8
+    lens = [3000 - 37 * b for b in range(24)]
+    kp, vp, table = filled(lay, lens, hkv, 33, width=25)
+    gen = tt.Generator("cuda").manual_seed(34)
+    q = tt.randn((24 * new, hq, D), generator=gen, device="cuda").half()
+    call = lambda: lay.paged_attention(hq, hkv)(q, kp, vp, table, ints(lens), cumulative([new] * 24), max_new=new)
+    want = call()
+    assert tt.isfinite(want).all()
+    for pool, codec in ((kp, lay.k_codec), (vp, lay.v_codec)):
+        for b, c in enumerate(lens):
+            if c % 128:
+                side = pool[int(table[b, c // 128])][:, 128 * (128 if codec is None else 16 * codec.bits):].view(tt.int16)
+                if codec is not None:
+                    side[:, c % 128:] = 0x7E00
+                elif pool is kp:
+                    side.view(hkv, 128, 4)[:, c % 128:] = 0x7E00
+                else:
+                    behind = (tt.arange(128, device="cuda") >= c % 128).view(1, 2, 1, 64)
+                    side.view(hkv, 2, 4, 64)[behind.expand(hkv, 2, 4, 64)] = 0x7E00
+    assert tt.equal(call(), want)
+
+
 def test_a_query_that_is_no_number_stays_in_its_row():
     lay, lens = layer("turbo3", "turbo4"), (500,)
     kp, vp, table = filled(lay, lens, 1, 18)
@@ -400,6 +443,37 @@ def test_two_captured_steps_of_different_plans_share_a_workspace():
         tt.cuda.synchronize()
         assert tt.equal(outs[turn], want[turn]), turn
         assert tt.equal(calls[1 - turn](tt.empty_like(outs[1 - turn])), want[1 - turn])
+
+
+def test_a_captured_step_outlives_its_workspace():
+    """A larger call replaces the object's workspace; what was captured with the smaller one still has it to itself."""
+    lay, lens = layer("turbo3", "turbo3"), (2000,)
+    kp, vp, table = filled(lay, lens, 1, 37)
+    q = tt.randn((8, 4, D), device="cuda").half()
+    n, cu = ints(lens), cumulative([8])
+    attn, out = lay.paged_attention(4, 1), tt.empty((1, 4, D), dtype=tt.float16, device="cuda")
+    call = lambda: attn(q[:1], kp, vp, table, n, max_context=2000, out=out)
+    side = tt.cuda.Stream()
+    side.wait_stream(tt.cuda.current_stream())
+    with tt.cuda.stream(side):
+        call()
+        side.synchronize()
+        graph = tt.cuda.CUDAGraph()
+        with tt.cuda.graph(graph, stream=side):
+            call()
+    tt.cuda.synchronize()
+    want, small = out.clone(), attn.workspace.numel()
+    wide = tt.zeros((1, 4000), dtype=tt.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    attn(q, kp, vp, wide, n, cu)        # positions up to 512 000 size it
+    assert attn.workspace.numel() > small
+    with tt.cuda.stream(side):          # what the allocator may hand out again
+        taken = [tt.full((small,), 1, dtype=tt.uint8, device="cuda") for _ in range(4)]
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        tt.cuda.synchronize()
+        assert tt.equal(out, want) and all((x == 1).all() for x in taken)
 
 
 @pytest.mark.parametrize("causal", [True, False])

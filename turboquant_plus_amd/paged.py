@@ -158,7 +158,7 @@ class PagedAttention:
         self.k_codec, self.v_codec = k_codec, v_codec
         self.n_q_heads, self.n_kv_heads, self.causal = n_q_heads, n_kv_heads, bool(causal)
         self.scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-        self.workspace, self._outgrown = None, []
+        self.workspace, self._spaces = None, {}      # the last call's; every device's, ever larger
 
     def __call__(self, q, k_pages, v_pages, block_table, lens, cu_new=None, *, max_context: int | None = None, max_new: int | None = None,
                  out=None):
@@ -189,12 +189,11 @@ class PagedAttention:
         need = lib.tq_paged_attn_workspace_bytes(at)
         if need < 0:
             L.check(L.ERR_ARG)
-        room = -1 if self.workspace is None or self.workspace.get_device() != device else self.workspace.numel()
-        if room < need:
-            if self.workspace is not None:
-                self._outgrown.append(self.workspace)     # a captured call may still write to it
-            self.workspace = tt.empty(need, dtype=tt.uint8, device=q.device)
-            room = need
+        spaces = self._spaces.get(device)
+        if spaces is None or spaces[-1].numel() < need:     # smaller ones stay: a captured call may still write to them
+            spaces = self._spaces.setdefault(device, [])
+            spaces.append(tt.empty(need, dtype=tt.uint8, device=q.device))
+        self.workspace = space = spaces[-1]
         L.check(lib.tq_paged_attention(_handle(self.k_codec), _handle(self.v_codec), at, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                                       out.data_ptr(), self.workspace.data_ptr(), room, L.stream_ptr()))
+                                       out.data_ptr(), space.data_ptr(), space.numel(), L.stream_ptr()))
         return out
