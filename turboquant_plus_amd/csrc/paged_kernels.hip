@@ -18,49 +18,78 @@ using namespace tqpaged;
 
 constexpr int MERGE_THREADS = 256;
 
-// The splits' partial results of a row -> its output: a wavefront per row and query head, two dims per lane.
+// The splits' partial results of a row -> its output: two dims per lane, a wavefront has HEADS query heads of a row with their reads in
+// flight together: it waits for the tables first (4 x 448 rows x 16 heads, two splits: one head each 15.5 us, four 11.8; 80 rows x 64 heads,
+// two splits: 4.9, 5.5).
+constexpr int MERGE_HEADS = 4;
 __global__ __launch_bounds__(MERGE_THREADS) void k_paged_merge(PagedAttnArgs a) {
-    const int lane = threadIdx.x & 63, heads = a.r.p.n_kv_heads * a.group;
+    const int lane = threadIdx.x & 63, heads = a.r.p.n_kv_heads * a.group, sets = (heads + MERGE_HEADS - 1) / MERGE_HEADS;
     const int64_t at = (int64_t)blockIdx.x * (MERGE_THREADS / 64) + (threadIdx.x >> 6);
-    const int64_t row = at / heads;
-    const int head = (int)(at - row * heads);
+    const int64_t row = at / sets;
+    const int head0 = (int)(at - row * sets) * MERGE_HEADS;
     if (row >= a.r.rows) return;
     int b, nth;
     PagedSeq seq;
     if (!paged_item(a.r, (int)row, [&](const PagedSeq &q) { return q.n; }, b, nth, seq)) return;
     const PagedSpan span = paged_span(a, seq);
     if (span.splits <= 1 || nth >= a.max_new) return;
-    const int64_t place = ((int64_t)(seq.row0 + nth) * heads + head) * a.n_splits;
-    float top = -INFINITY;
-    for (int s = lane; s < span.splits; s += 64) top = fmaxf(top, a.part_ml[2 * (place + s)]);
+    const int64_t out_row = (int64_t)(seq.row0 + nth) * heads;
+    int64_t place[MERGE_HEADS];
+    float top[MERGE_HEADS];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float off = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-#pragma unroll 4
+    for (int h = 0; h < MERGE_HEADS; ++h) {   // heads past the last one repeat it
+        place[h] = (out_row + min(head0 + h, heads - 1)) * a.n_splits;
+        top[h] = -INFINITY;
+    }
+    for (int s = lane; s < span.splits; s += 64)
+#pragma unroll
+        for (int h = 0; h < MERGE_HEADS; ++h) top[h] = fmaxf(top[h], a.part_ml[2 * (place[h] + s)]);
+#pragma unroll
+    for (int h = 0; h < MERGE_HEADS; ++h) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top[h] = fmaxf(top[h], __shfl_xor(top[h], o));
+        top[h] = top[h] == -INFINITY ? 0.0f : top[h];
+    }
+    float l[MERGE_HEADS] = {}, o0[MERGE_HEADS] = {}, o1[MERGE_HEADS] = {};
+#pragma unroll 2
     for (int s = 0; s < span.splits; ++s) {
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (place + s));
-        const float2 v = *reinterpret_cast<const float2 *>(a.part_o + (place + s) * 128 + 2 * lane);
-        const float f = __builtin_amdgcn_exp2f(ml.x - off);
-        l = fmaf(ml.y, f, l);
-        o0 = fmaf(v.x, f, o0);
-        o1 = fmaf(v.y, f, o1);
+        float2 ml[MERGE_HEADS], v[MERGE_HEADS];
+#pragma unroll
+        for (int h = 0; h < MERGE_HEADS; ++h) {
+            ml[h] = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (place[h] + s));
+            v[h] = *reinterpret_cast<const float2 *>(a.part_o + (place[h] + s) * 128 + 2 * lane);
+        }
+#pragma unroll
+        for (int h = 0; h < MERGE_HEADS; ++h) {
+            const float f = __builtin_amdgcn_exp2f(ml[h].x - top[h]);
+            l[h] = fmaf(ml[h].y, f, l[h]);
+            o0[h] = fmaf(v[h].x, f, o0[h]);
+            o1[h] = fmaf(v[h].y, f, o1[h]);
+        }
     }
-    float inv = l > 0.0f ? a.v_unscale / l : l == 0.0f ? 0.0f : l;
+    float2 s1 = make_float2(1.0f, 1.0f), s2 = s1;
     if (a.vs1) {
-        const float2 s1 = *reinterpret_cast<const float2 *>(a.vs1 + 2 * lane), s2 = *reinterpret_cast<const float2 *>(a.vs2 + 2 * lane);
-        o0 *= s2.x;
-        o1 *= s2.y;
-        wht128_wave(o0, o1, lane);
-        o0 *= s1.x;
-        o1 *= s1.y;
-        inv *= RSQRT128;
+        s1 = *reinterpret_cast<const float2 *>(a.vs1 + 2 * lane);
+        s2 = *reinterpret_cast<const float2 *>(a.vs2 + 2 * lane);
     }
-    o0 *= inv;
-    o1 *= inv;
-    const uint32_t lo = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o0) : __builtin_bit_cast(uint16_t, (_Float16)o0);
-    const uint32_t hi = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o1) : __builtin_bit_cast(uint16_t, (_Float16)o1);
-    reinterpret_cast<uint32_t *>(a.out)[((int64_t)(seq.row0 + nth) * heads + head) * 64 + lane] = lo | (hi << 16);
+#pragma unroll
+    for (int h = 0; h < MERGE_HEADS; ++h) {
+        if (head0 + h >= heads) return;
+        float inv = l[h] > 0.0f ? a.v_unscale / l[h] : l[h] == 0.0f ? 0.0f : l[h], x0 = o0[h], x1 = o1[h];
+        if (a.vs1) {
+            x0 *= s2.x;
+            x1 *= s2.y;
+            wht128_wave(x0, x1, lane);
+            x0 *= s1.x;
+            x1 *= s1.y;
+            inv *= RSQRT128;
+        }
+        x0 *= inv;
+        x1 *= inv;
+        const uint32_t lo = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)x0) : __builtin_bit_cast(uint16_t, (_Float16)x0);
+        const uint32_t hi = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)x1) : __builtin_bit_cast(uint16_t, (_Float16)x1);
+        reinterpret_cast<uint32_t *>(a.out)[(out_row + head0 + h) * 64 + lane] = lo | (hi << 16);
+    }
 }
 
 struct Plan {
@@ -73,6 +102,7 @@ struct Plan {
     int hg, wpw, gpw, parts, passes, wg_tiles, splits;
 };
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t merge_groups(const tq_paged_attn_params *p) { return ceil_div(p->rows * ceil_div(p->n_q_heads, MERGE_HEADS), MERGE_THREADS / 64); }
 struct Formats {
     int kb, vb;    // code widths, 8 for 8-bit rows
     bool share;    // one codebook
@@ -147,7 +177,7 @@ bool make_plan(const tq_paged_attn_params *p, const Formats &f, Plan &pl) {
     pl.split_tiles = (int)ceil_div(tiles, splits);
     pl.n_splits = (int)ceil_div(tiles, pl.split_tiles);
     const int64_t grid = ceil_div(pl.items, w / pl.kw) * pl.n_splits * p->pages.n_kv_heads;
-    if (grid > 0x7FFFFFFF || rows * group > 0x7FFFFFFF || ceil_div(rows * p->n_q_heads, MERGE_THREADS / 64) > 0x7FFFFFFF) return false;
+    if (grid > 0x7FFFFFFF || rows * group > 0x7FFFFFFF || merge_groups(p) > 0x7FFFFFFF) return false;
     pl.grid = (unsigned)grid;
     return true;
 }
@@ -334,7 +364,7 @@ int tq_paged_attention(const tq_handle *hk, const tq_handle *hv, const tq_paged_
     default: rc = tqk_paged_attn_k8(a, vb, pl.kind, pl.grid, s); break;
     }
     if (rc || pl.n_splits == 1) return rc;
-    k_paged_merge<<<(unsigned)ceil_div(p->rows * p->n_q_heads, MERGE_THREADS / 64), MERGE_THREADS, 0, s>>>(a);
+    k_paged_merge<<<(unsigned)merge_groups(p), MERGE_THREADS, 0, s>>>(a);
     return tq_check_launch("paged_merge");
 }
 
