@@ -572,6 +572,28 @@ def test_pools_beyond_32_bits():
                                               lay.load_paged(*small, near, ints([0]), cumulative([300]), 300)))
 
 
+@pytest.mark.parametrize("kf,vf", [("q8_0", "turbo4"), ("turbo4", "turbo4")])
+def test_few_rows_in_pools_beyond_32_bits(kf, vf):
+    """The other kernels: single tokens with and without 4-bit tables of a copy per lane, 16, 24, 48 and 60 rows."""
+    lay, hkv, c = layer(kf, vf), 8, 3000
+    n = int(4.5 * 2 ** 30) // (hkv * 128 * 66)
+    kp, vp = lay.new_pages(n, hkv)
+    blocks = -(-c // 128)
+    small = lay.new_pages(blocks, hkv)
+    table, near = ints([[n - 1 - i for i in range(blocks)]]), ints([list(range(blocks))])
+    k, v = (tt.randn((c, hkv, D), device="cuda").half() for _ in range(2))
+    lay.append_paged(k, v, kp, vp, table, ints([0]), cumulative([c]))
+    lay.append_paged(k, v, *small, near, ints([0]), cumulative([c]))
+    attn = lay.paged_attention(16, hkv)
+    for new in (1, 8, 12, 24, 30):
+        q = tt.randn((new, 16, D), device="cuda").half()
+        assert tt.equal(attn(q, kp, vp, table, ints([c]), cumulative([new])), attn(q, *small, near, ints([c]), cumulative([new]))), new
+    many = 32
+    q = tt.randn((many, 16, D), device="cuda").half()      # a prefix that all of a batch share
+    got, want = (attn(q, *pools, rows.expand(many, blocks).contiguous(), ints([c] * many)) for pools, rows in (((kp, vp), table), (small, near)))
+    assert tt.equal(got, want)
+
+
 # ---- a serving loop --------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kf,vf", [("turbo3", "turbo3"), ("q8_0", "turbo4")])
